@@ -96,6 +96,65 @@ int llamini_gemv_device(u32 type, const void* d_w, u32 rows, u32 cols,
 int llamini_causal_mha_noalloc(const f32* d_q, const f32* d_key, const f32* d_val, f32* d_out,
                                u32 pos, u32 n_heads, u32 n_heads_kv, u32 head_dim, void* stream);
 
+/* ---- 8-bit integer operators (no counterpart in the reference, whose products
+ *      decode each weight to f32: model.c:66-176) ------------------------------
+ *
+ * A decoder layer's matrices as int8 x int8 products on the tensor cores: int8
+ * weights with one scale for each output channel, activations with one scale
+ * for each token. A row q[0..cols) with its scale stands for the values
+ * q[i] * scale, where scale = max|y| / 127 and q = y / scale rounded to the
+ * nearest integer, ties to even. A row of zeros has scale 0; a row that holds a
+ * NaN or an infinity has scale NaN and q = 0.
+ *
+ * Every call takes DEVICE buffers of the calling thread's current device (others
+ * are refused) and enqueues its work on `stream` (a cudaStream_t; NULL = the
+ * legacy default stream). None allocates, keeps anything from call to call or
+ * uses scratch, so calls may overlap in time and may be captured into graphs.
+ * Matrices are row-major; a pitch ld_* counts elements from row to row and is at
+ * least the row's length. What lies between a row's end and the next row's start
+ * is neither read nor written. Pitches in multiples of 16 elements from a 16-byte
+ * aligned base are what the fast kernels take; other ones work, slower. 1 to
+ * 131071 columns; rows = 0 is a call without work. Outputs must not overlap
+ * inputs, but for the sum of llamini_rms_norm_i8_device. */
+
+/* Element types of activations: GGML_TYPE_F32, GGML_TYPE_F16 and */
+#define LLAMINI_TYPE_BF16 30
+
+/* Activations of llamini_glu_i8_device: ACT_SILU, ACT_GELU (model.h) and */
+#define LLAMINI_ACT_NONE 2
+
+/* int8 rows of raw GGUF blocks: the `cols` elements of each of `rows` rows,
+ * decoded as by llamini_dequant_device (bit-identical to gguf.c:409-594), get
+ * the row's scale; q is the exact nearest integer of w / scale. d_blocks holds
+ * whole rows back to back (2-byte aligned; F32 4-byte), d_q is rows x ld_q, d_scale
+ * holds `rows` floats. Done once per matrix, when a model is loaded. */
+int llamini_weights_i8_device(u32 type, const void* d_blocks, u32 rows, u32 cols,
+                              i8* d_q, u64 ld_q, f32* d_scale, void* stream);
+
+/* RMS norm of each row with the residual's addition, rounded to int8:
+ * h = x + resid in f32 (x alone when d_resid is NULL), y = h / sqrt(mean(h^2) +
+ * eps) * w (rms_norm, model.c:4-10), q and scale of y. x, resid and sum are of
+ * `type`. d_sum (NULL: not stored) receives h rounded to `type`; it may be d_x or
+ * d_resid, with that input's pitch, to update a residual stream in place. d_w
+ * holds `cols` floats. */
+int llamini_rms_norm_i8_device(u32 type, const void* d_x, u64 ld_x, const void* d_resid, u64 ld_resid,
+                               void* d_sum, u64 ld_sum, const f32* d_w, f32 eps, u32 rows, u32 cols,
+                               i8* d_q, u64 ld_q, f32* d_scale, void* stream);
+
+/* y = act(gate) * up, or act(gate) when d_up is NULL (ffn_glu, model.c:14-25;
+ * with LLAMINI_ACT_NONE and no up, the rounding of plain rows to int8), q and
+ * scale of y. gate and up are of `type` and may lie side by side in one buffer,
+ * as one product of both matrices leaves them. */
+int llamini_glu_i8_device(u32 type, const void* d_gate, u64 ld_gate, const void* d_up, u64 ld_up, u32 act,
+                          u32 rows, u32 cols, i8* d_q, u64 ld_q, f32* d_scale, void* stream);
+
+/* out[m][j] = (sum_k a[m][k] w[j][k]) * a_scale[m] * w_scale[j] (+ bias[j]) for
+ * m < rows, j < n: the sum exact in 32-bit integers, the rest in f32, rounded to
+ * out_type (F32, F16, BF16). d_bias may be NULL. a is rows x cols, w n x cols. */
+int llamini_gemm_i8_device(const i8* d_a, u64 ld_a, const f32* d_a_scale, u32 rows,
+                           const i8* d_w, u64 ld_w, const f32* d_w_scale, u32 n, u32 cols,
+                           const f32* d_bias, u32 out_type, void* d_out, u64 ld_out, void* stream);
+
 /* ---- device-resident decoding sessions (generate.c:122-167 without host
  *      round trips) --------------------------------------------------------- */
 

@@ -177,6 +177,10 @@ SIGNATURES = {
     "llamini_session_kv_bytes_per_pos": (u64, [P]),
     "llamini_set_kv_f16": (C.c_int, [C.c_int]),
     "llamini_causal_mha_noalloc": (C.c_int, [P, P, P, P, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, P]),
+    "llamini_weights_i8_device": (C.c_int, [u32, P, u32, u32, P, u64, P, P]),
+    "llamini_rms_norm_i8_device": (C.c_int, [u32, P, u64, P, u64, P, u64, P, f32, u32, u32, P, u64, P, P]),
+    "llamini_glu_i8_device": (C.c_int, [u32, P, u64, P, u64, u32, u32, u32, P, u64, P, P]),
+    "llamini_gemm_i8_device": (C.c_int, [P, u64, P, u32, P, u64, P, u32, u32, P, u32, P, u64, P]),
     "llamini_session_trace": (C.c_int, [P, C.c_int]),
     "llamini_session_trace_read": (C.c_int, [P, P]),
 }

@@ -1,0 +1,452 @@
+// k_i8.cu -- rows of int8 with one scale each: from GGUF blocks (weights), from
+// an RMS norm with the residual's addition, and from a gated activation. They
+// feed the int8 matrix product in k_gemm_i8.cu.
+//
+// Each operator is two passes over a row: the largest magnitude (and for the
+// norm the sum of squares), then the rounding to int8 (i8.cuh). Sums, scales
+// and every value before the rounding are f32.
+#include "i8.cuh"
+
+namespace lm {
+namespace {
+
+// ---------------------------------------------------------------- norm
+
+struct NormArgs {
+    const void* x;
+    const void* resid;         // may be null
+    void* sum;                 // may be null; may be x or resid with its pitch
+    const float* w;
+    int8_t* q;
+    float* scale;
+    uint64_t ld_x, ld_resid, ld_sum, ld_q;
+    uint32_t rows, cols;
+    float eps;
+};
+
+// h = x + resid in f32 (its rounding to the type is only for the stored sum),
+// y = h / sqrt(mean(h^2) + eps) * w. One CTA a row. Each thread reads an
+// element before the same thread overwrites it, in the second pass, so the sum
+// may be stored over x or the residual.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_i8_kernel(const NormArgs a) {
+    __shared__ uint32_t red[64];
+    const uint64_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
+    const T* r = a.resid ? static_cast<const T*>(a.resid) + row * a.ld_resid : nullptr;
+    T* o = a.sum ? static_cast<T*>(a.sum) + row * a.ld_sum : nullptr;
+    uint32_t m = 0;
+    float ss = 0.f;
+    for (uint32_t i = threadIdx.x; i < a.cols; i += blockDim.x) {
+        const float h = to_f32(x[i]) + (r ? to_f32(r[i]) : 0.f);
+        ss = fmaf(h, h, ss);
+        m = max(m, abs_bits(h * a.w[i]));
+    }
+    block_max_sum(m, ss, red);
+    const float rstd = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
+    const RowScale s = row_scale(__uint_as_float(m) * rstd);
+    for (uint32_t i = threadIdx.x; i < a.cols; i += blockDim.x) {
+        const float h = to_f32(x[i]) + (r ? to_f32(r[i]) : 0.f);
+        if (o) o[i] = from_f32<T>(h);
+        a.q[row * a.ld_q + i] = (int8_t)quant1(h * a.w[i] * rstd, s);
+    }
+    if (threadIdx.x == 0) a.scale[row] = s.scale;
+}
+
+// ---------------------------------------------------------------- gated activation
+
+struct GluArgs {
+    const void* gate;
+    const void* up;            // may be null: act(gate) alone
+    int8_t* q;
+    float* scale;
+    uint64_t ld_gate, ld_up, ld_q;
+    uint32_t rows, cols, act;
+};
+
+// The activations of model.c:14-25 (and gpt2.c's gelu), in f32.
+template <uint32_t ACT>
+__device__ __forceinline__ float activate(float x) {
+    if (ACT == ACT_SILU) return x / (1.0f + expf(-x));
+    if (ACT == ACT_GELU) {
+        const float k0 = 0.79788456080286535587989211986876f;
+        return 0.5f * x * (1.0f + tanhf(k0 * x * (1.0f + 0.044715f * x * x)));
+    }
+    return x;
+}
+
+template <typename T, uint32_t ACT>
+__global__ void __launch_bounds__(256) glu_i8_kernel(const GluArgs a) {
+    __shared__ uint32_t red[64];
+    const uint64_t row = blockIdx.x;
+    const T* g = static_cast<const T*>(a.gate) + row * a.ld_gate;
+    const T* u = a.up ? static_cast<const T*>(a.up) + row * a.ld_up : nullptr;
+    uint32_t m = 0;
+    float unused = 0.f;
+    for (uint32_t i = threadIdx.x; i < a.cols; i += blockDim.x)
+        m = max(m, abs_bits(activate<ACT>(to_f32(g[i])) * (u ? to_f32(u[i]) : 1.f)));
+    block_max_sum(m, unused, red);
+    const RowScale s = row_scale(__uint_as_float(m));
+    for (uint32_t i = threadIdx.x; i < a.cols; i += blockDim.x)
+        a.q[row * a.ld_q + i] = (int8_t)quant1(activate<ACT>(to_f32(g[i])) * (u ? to_f32(u[i]) : 1.f), s);
+    if (threadIdx.x == 0) a.scale[row] = s.scale;
+}
+
+// ---------------------------------------------------------------- weights
+
+struct WeightArgs {
+    const uint8_t* raw;
+    int8_t* q;
+    float* scale;
+    uint64_t row_bytes, ld_q;
+    uint32_t rows, cols, type;
+    uint32_t seg_units;        // units of a segment of a row that fits shared memory
+};
+
+constexpr uint32_t kWSeg = 48 * 1024;      // raw bytes of a row staged at a time
+constexpr uint32_t kWSlack = 192;          // behind it: the offset modulo 16, and a short last unit decoded whole
+constexpr uint32_t kWThreads = 256;
+
+
+// NW little-endian words from a 2-byte aligned address in shared memory (the
+// aligned words around it; reads up to two bytes past the range).
+template <int NW>
+__device__ __forceinline__ void words_at(const uint8_t* p, uint32_t* w) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+    const uint32_t* b = reinterpret_cast<const uint32_t*>(a & ~uintptr_t(3));
+    const uint32_t s = (uint32_t)(a & 2u) * 8u;
+    uint32_t prev = b[0];
+#pragma unroll
+    for (int i = 0; i < NW; i++) {
+        const uint32_t nx = b[i + 1];
+        w[i] = __funnelshift_r(prev, nx, s);
+        prev = nx;
+    }
+}
+__device__ __forceinline__ float half_at(const uint8_t* p) {
+    return __half2float(*reinterpret_cast<const __half*>(p));
+}
+__device__ __forceinline__ uint32_t byte_at(const uint32_t* w, int i) { return (w[i >> 2] >> ((i & 3) * 8)) & 0xFFu; }
+
+// Elements 32 u .. 32 u + 31 of a row whose bytes (from the first block of
+// the staged segment on) are at `row`, in their own order, bit-identical to gguf.c:409-594:
+// each product and sum is rounded on its own.
+template <uint32_t T>
+__device__ __forceinline__ void unit_weights(const uint8_t* row, uint32_t u, float* y) {
+    uint32_t w[8];
+    if constexpr (T == GGML_TYPE_Q8_0) {
+        const uint8_t* b = row + (size_t)u * 34;
+        const float d = half_at(b);
+        words_at<8>(b + 2, w);
+#pragma unroll
+        for (int i = 0; i < 32; i++) y[i] = __fmul_rn((float)(int8_t)byte_at(w, i), d);
+    } else if constexpr (T == GGML_TYPE_Q4_0) {
+        const uint8_t* b = row + (size_t)u * 18;
+        const float d = half_at(b);
+        words_at<4>(b + 2, w);
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            y[i] = __fmul_rn((float)(int)(byte_at(w, i) & 15u) - 8.0f, d);
+            y[i + 16] = __fmul_rn((float)(int)(byte_at(w, i) >> 4) - 8.0f, d);
+        }
+    } else if constexpr (T == GGML_TYPE_Q4_1) {
+        const uint8_t* b = row + (size_t)u * 20;
+        const float d = half_at(b), m = half_at(b + 2);
+        words_at<4>(b + 4, w);
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            y[i] = __fadd_rn(__fmul_rn((float)(byte_at(w, i) & 15u), d), m);
+            y[i + 16] = __fadd_rn(__fmul_rn((float)(byte_at(w, i) >> 4), d), m);
+        }
+    } else if constexpr (T == GGML_TYPE_Q5_0) {
+        const uint8_t* b = row + (size_t)u * 22;
+        const float d = half_at(b);
+        words_at<5>(b + 2, w);
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const uint32_t lo = (byte_at(w + 1, i) & 15u) | (((w[0] >> i) & 1u) << 4);
+            const uint32_t hi = (byte_at(w + 1, i) >> 4) | (((w[0] >> (i + 16)) & 1u) << 4);
+            y[i] = __fmul_rn((float)lo - 16.0f, d);
+            y[i + 16] = __fmul_rn((float)hi - 16.0f, d);
+        }
+    } else if constexpr (T == GGML_TYPE_Q4_K || T == GGML_TYPE_Q5_K) {
+        constexpr bool five = T == GGML_TYPE_Q5_K;
+        const uint8_t* b = row + (size_t)(u >> 3) * (five ? 176 : 144);
+        const uint32_t j = u & 7u;
+        const float d = half_at(b), dmin = half_at(b + 2);
+        const uint8_t* sc = b + 4;
+        uint32_t s6, m6;                             // gguf.c:391-399
+        if (j < 4) {
+            s6 = sc[j] & 63u;
+            m6 = sc[j + 4] & 63u;
+        } else {
+            s6 = (sc[j + 4] & 15u) | ((uint32_t)(sc[j - 4] >> 6) << 4);
+            m6 = (sc[j + 4] >> 4) | ((uint32_t)(sc[j] >> 6) << 4);
+        }
+        const float ds = __fmul_rn(d, (float)s6), dm = __fmul_rn(dmin, (float)m6);
+        words_at<8>(b + (five ? 48 : 16) + 32 * (j >> 1), w);
+        uint32_t h[8];
+        if constexpr (five) words_at<8>(b + 16, h);
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+            uint32_t v = (byte_at(w, i) >> (4 * (j & 1u))) & 15u;
+            if constexpr (five) v |= ((byte_at(h, i) >> j) & 1u) << 4;
+            y[i] = __fsub_rn(__fmul_rn(ds, (float)v), dm);
+        }
+    } else if constexpr (T == GGML_TYPE_Q6_K) {
+        const uint8_t* b = row + (size_t)(u >> 3) * 210;
+        const uint32_t j = u & 7u, p = j >> 2, c = j & 3u;
+        const float d = half_at(b + 208);
+        uint32_t h[8];
+        words_at<8>(b + 64 * p + 32 * (c & 1u), w);
+        words_at<8>(b + 128 + 32 * p, h);
+        const int8_t* sc = reinterpret_cast<const int8_t*>(b + 192 + 8 * p + 2 * c);
+        const float d0 = __fmul_rn(d, (float)sc[0]), d1 = __fmul_rn(d, (float)sc[1]);
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+            const int v = (int)(((byte_at(w, i) >> (4 * (c >> 1))) & 15u) | (((byte_at(h, i) >> (2 * c)) & 3u) << 4)) - 32;
+            y[i] = __fmul_rn(i < 16 ? d0 : d1, (float)v);
+        }
+    } else if constexpr (T == GGML_TYPE_F16) {
+        const __half* b = reinterpret_cast<const __half*>(row) + (size_t)u * 32;
+#pragma unroll
+        for (int i = 0; i < 32; i++) y[i] = __half2float(b[i]);
+    } else {
+        const float* b = reinterpret_cast<const float*>(row) + (size_t)u * 32;
+#pragma unroll
+        for (int i = 0; i < 32; i++) y[i] = b[i];
+    }
+}
+
+__host__ __device__ constexpr uint32_t block_elems(uint32_t t) {
+    return t == GGML_TYPE_F32 || t == GGML_TYPE_F16 ? 1 : t >= GGML_TYPE_Q4_K ? 256 : 32;
+}
+__host__ __device__ constexpr uint32_t block_bytes(uint32_t t) {
+    return t == GGML_TYPE_F32 ? 4 : t == GGML_TYPE_F16 ? 2 : t == GGML_TYPE_Q4_0 ? 18 : t == GGML_TYPE_Q4_1 ? 20
+         : t == GGML_TYPE_Q5_0 ? 22 : t == GGML_TYPE_Q8_0 ? 34 : t == GGML_TYPE_Q4_K ? 144
+         : t == GGML_TYPE_Q5_K ? 176 : 210;
+}
+
+// w / s rounded to the nearest integer, ties to even, exactly: the estimate
+// w * (127 / max) is within one of it, and the remainder w - q s comes from one
+// fused multiply-add, exact near s / 2 (there it is a multiple of half an ulp
+// of s and below s). Load-time work, so the int8 weights of a file are the
+// same everywhere.
+__device__ __forceinline__ int quant_exact(float w, const RowScale& r) {
+    if (r.zero || r.tiny) return quant1(w, r);
+    int q = __float2int_rn(w * r.inv);
+    const float rem = fmaf(-(float)q, r.scale, w), half = 0.5f * r.scale;
+    if (rem > half || (rem == half && (q & 1))) q++;
+    else if (rem < -half || (rem == -half && (q & 1))) q--;
+    return q;
+}
+
+// Segment `s0` (units) of a row into shared memory, at the same offset modulo
+// 16 as in global memory so that its middle moves in 16-byte words; nothing
+// outside the segment's bytes is read.
+__device__ __forceinline__ const uint8_t* stage_segment(uint8_t* sm, const uint8_t* src, uint32_t n) {
+    const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(src) & 15u);
+    const uint32_t head = min(n, (16u - off) & 15u), vecs = (n - head) / 16, tail = n - head - vecs * 16;
+    uint8_t* dst = sm + off;
+    for (uint32_t i = threadIdx.x; i < head + tail; i += blockDim.x) {
+        const uint32_t at = i < head ? i : head + vecs * 16 + (i - head);
+        dst[at] = src[at];
+    }
+    const uint4* v = reinterpret_cast<const uint4*>(src + head);
+    uint4* d = reinterpret_cast<uint4*>(dst + head);
+    for (uint32_t i = threadIdx.x; i < vecs; i += blockDim.x) d[i] = v[i];
+    __syncthreads();
+    return dst;
+}
+
+template <uint32_t T>
+__global__ void __launch_bounds__(kWThreads) weights_i8_kernel(const WeightArgs a) {
+    extern __shared__ __align__(16) uint8_t sm[];
+    __shared__ uint32_t red[64];
+    constexpr uint32_t BE = block_elems(T), BB = block_bytes(T);
+    const uint64_t row = blockIdx.x;
+    const uint8_t* src = a.raw + row * a.row_bytes;
+    int8_t* q = a.q + row * a.ld_q;
+    const uint32_t units = (a.cols + 31) / 32;       // the last one may be short (F32, F16)
+    const bool whole = units <= a.seg_units;
+    uint32_t m = 0;
+    float unused = 0.f;
+    RowScale rs = {};
+    for (uint32_t pass = 0; pass < 2; pass++) {
+        for (uint32_t u0 = 0; u0 < units; u0 += a.seg_units) {
+            const uint32_t nu = min(a.seg_units, units - u0), e0 = u0 * 32, ne = min(nu * 32, a.cols - e0);
+            const uint8_t* p = sm + (reinterpret_cast<uintptr_t>(src) & 15u);
+            if (pass == 0 || !whole) {
+                __syncthreads();                     // the segment before has been read
+                p = stage_segment(sm, src + (uint64_t)e0 / BE * BB, ne / BE * BB);
+            }
+            for (uint32_t u = threadIdx.x; u < nu; u += kWThreads) {
+                float y[32];
+                unit_weights<T>(p, u, y);
+                const uint32_t n = min(32u, ne - u * 32);
+#pragma unroll
+                for (uint32_t i = 0; i < 32; i++) {
+                    if (i >= n) break;
+                    if (pass == 0) m = max(m, abs_bits(y[i]));
+                    else q[e0 + u * 32 + i] = (int8_t)quant_exact(y[i], rs);
+                }
+            }
+        }
+        if (pass == 0) {
+            block_max_sum(m, unused, red);
+            rs = row_scale(__uint_as_float(m));
+        }
+    }
+    if (threadIdx.x == 0) a.scale[row] = rs.scale;
+}
+
+template <uint32_t T>
+bool launch_weights(const WeightArgs& a, cudaStream_t st) {
+    const uint32_t smem = (uint32_t)(a.row_bytes < kWSeg ? a.row_bytes : kWSeg) + kWSlack;
+    if (smem > 48 * 1024 &&
+        !LM_CUDA(cudaFuncSetAttribute(weights_i8_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kWSeg + kWSlack))))
+        return false;
+    weights_i8_kernel<T><<<a.rows, kWThreads, smem, st>>>(a);
+    return LM_CUDA(cudaGetLastError());
+}
+
+bool act_type_ok(const char* who, uint32_t type) {
+    if (act_bytes(type)) return true;
+    set_error("%s: element type %u is not F32, F16 or BF16", who, type);
+    return false;
+}
+bool cols_ok(const char* who, uint32_t cols) {
+    if (cols >= 1 && cols <= kI8MaxCols) return true;
+    set_error("%s: %u columns (1 to %u)", who, cols, kI8MaxCols);
+    return false;
+}
+bool pitch_ok(const char* who, const char* what, u64 ld, uint32_t cols) {
+    if (ld >= cols && ld <= (1ull << 40)) return true;
+    set_error("%s: pitch %llu of %s for %u columns", who, (unsigned long long)ld, what, cols);
+    return false;
+}
+bool rows_ok(const char* who, uint32_t rows) {
+    if (rows <= 0x7FFFFFFFu) return true;
+    set_error("%s: %u rows (at most 2^31 - 1)", who, rows);
+    return false;
+}
+bool align_ok(const char* who, const void* const* ptrs, int n, size_t bytes) {
+    for (int i = 0; i < n; i++)
+        if (ptrs[i] && !i8_aligned(ptrs[i], bytes)) {
+            set_error("%s: an array of %u-byte elements is not aligned to them", who, (unsigned)bytes);
+            return false;
+        }
+    return true;
+}
+
+template <typename T>
+bool launch_glu(const GluArgs& a, cudaStream_t st) {
+    if (a.act == ACT_SILU) glu_i8_kernel<T, ACT_SILU><<<a.rows, 256, 0, st>>>(a);
+    else if (a.act == ACT_GELU) glu_i8_kernel<T, ACT_GELU><<<a.rows, 256, 0, st>>>(a);
+    else glu_i8_kernel<T, LLAMINI_ACT_NONE><<<a.rows, 256, 0, st>>>(a);
+    return LM_CUDA(cudaGetLastError());
+}
+template <typename T>
+bool launch_norm(const NormArgs& a, cudaStream_t st) {
+    norm_i8_kernel<T><<<a.rows, 256, 0, st>>>(a);
+    return LM_CUDA(cudaGetLastError());
+}
+
+}  // namespace
+}  // namespace lm
+
+extern "C" int llamini_weights_i8_device(u32 type, const void* d_blocks, u32 rows, u32 cols, i8* d_q, u64 ld_q,
+                                         f32* d_scale, void* stream) {
+    using namespace lm;
+    const char* who = "weights_i8";
+    TypeInfo ti;
+    if (!type_info(type, &ti)) { set_error("%s: unsupported type %u", who, type); return -1; }
+    if (!cols_ok(who, cols) || !rows_ok(who, rows) || !pitch_ok(who, "q", ld_q, cols)) return -1;
+    if (cols % ti.block_elems != 0) {
+        set_error("%s: %u columns are not whole blocks of type %u", who, cols, type);
+        return -1;
+    }
+    if (rows == 0) return 0;
+    const void* ptrs[] = {d_blocks, d_q, d_scale};
+    if (!d_blocks || !d_q || !d_scale) { set_error("%s: null pointer", who); return -1; }
+    const size_t align = type == GGML_TYPE_F32 ? 4 : 2;      // blocks start with, and are read in, 16-bit fields
+    if (!align_ok(who, ptrs, 1, align) || !align_ok(who, ptrs + 2, 1, 4) || !i8_device_ptrs(who, ptrs, 3)) return -1;
+    WeightArgs a;
+    a.raw = static_cast<const uint8_t*>(d_blocks);
+    a.q = reinterpret_cast<int8_t*>(d_q);
+    a.scale = d_scale;
+    a.row_bytes = type_bytes(type, cols);
+    a.ld_q = ld_q;
+    a.rows = rows; a.cols = cols; a.type = type;
+    // whole blocks, and whole 32-element units, to a segment
+    const uint32_t per = ti.block_elems >= 32 ? ti.block_elems : 32;
+    a.seg_units = kWSeg / (per / ti.block_elems * ti.block_bytes) * (per / 32);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    bool ok = false;
+    switch (type) {
+    case GGML_TYPE_F32: ok = launch_weights<GGML_TYPE_F32>(a, st); break;
+    case GGML_TYPE_F16: ok = launch_weights<GGML_TYPE_F16>(a, st); break;
+    case GGML_TYPE_Q4_0: ok = launch_weights<GGML_TYPE_Q4_0>(a, st); break;
+    case GGML_TYPE_Q4_1: ok = launch_weights<GGML_TYPE_Q4_1>(a, st); break;
+    case GGML_TYPE_Q5_0: ok = launch_weights<GGML_TYPE_Q5_0>(a, st); break;
+    case GGML_TYPE_Q8_0: ok = launch_weights<GGML_TYPE_Q8_0>(a, st); break;
+    case GGML_TYPE_Q4_K: ok = launch_weights<GGML_TYPE_Q4_K>(a, st); break;
+    case GGML_TYPE_Q5_K: ok = launch_weights<GGML_TYPE_Q5_K>(a, st); break;
+    case GGML_TYPE_Q6_K: ok = launch_weights<GGML_TYPE_Q6_K>(a, st); break;
+    }
+    return ok ? 0 : -1;
+}
+
+extern "C" int llamini_rms_norm_i8_device(u32 type, const void* d_x, u64 ld_x, const void* d_resid, u64 ld_resid,
+                                          void* d_sum, u64 ld_sum, const f32* d_w, f32 eps, u32 rows, u32 cols,
+                                          i8* d_q, u64 ld_q, f32* d_scale, void* stream) {
+    using namespace lm;
+    const char* who = "rms_norm_i8";
+    if (!act_type_ok(who, type) || !cols_ok(who, cols) || !rows_ok(who, rows) || !pitch_ok(who, "x", ld_x, cols) ||
+        (d_resid && !pitch_ok(who, "the residual", ld_resid, cols)) ||
+        (d_sum && !pitch_ok(who, "the sum", ld_sum, cols)) || !pitch_ok(who, "q", ld_q, cols))
+        return -1;
+    if (!(eps >= 0.0f)) { set_error("%s: eps is negative or NaN", who); return -1; }
+    if ((d_sum == d_x && d_x && ld_sum != ld_x) || (d_sum && d_sum == d_resid && ld_sum != ld_resid)) {
+        set_error("%s: a sum stored over its input needs that input's pitch", who);
+        return -1;
+    }
+    if (rows == 0) return 0;
+    const void* ptrs[] = {d_x, d_resid, d_sum, d_w, d_q, d_scale};
+    if (!d_x || !d_w || !d_q || !d_scale) { set_error("%s: null pointer", who); return -1; }
+    const void* f32s[] = {d_w, d_scale};
+    if (!align_ok(who, ptrs, 3, act_bytes(type)) || !align_ok(who, f32s, 2, 4) || !i8_device_ptrs(who, ptrs, 6)) return -1;
+    NormArgs a;
+    a.x = d_x; a.resid = d_resid; a.sum = d_sum; a.w = d_w;
+    a.q = reinterpret_cast<int8_t*>(d_q); a.scale = d_scale;
+    a.ld_x = ld_x; a.ld_resid = ld_resid; a.ld_sum = ld_sum; a.ld_q = ld_q;
+    a.rows = rows; a.cols = cols; a.eps = eps;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool ok = type == GGML_TYPE_F32 ? launch_norm<float>(a, st)
+                  : type == GGML_TYPE_F16 ? launch_norm<__half>(a, st) : launch_norm<__nv_bfloat16>(a, st);
+    return ok ? 0 : -1;
+}
+
+extern "C" int llamini_glu_i8_device(u32 type, const void* d_gate, u64 ld_gate, const void* d_up, u64 ld_up, u32 act,
+                                     u32 rows, u32 cols, i8* d_q, u64 ld_q, f32* d_scale, void* stream) {
+    using namespace lm;
+    const char* who = "glu_i8";
+    if (!act_type_ok(who, type) || !cols_ok(who, cols) || !rows_ok(who, rows) ||
+        !pitch_ok(who, "gate", ld_gate, cols) || (d_up && !pitch_ok(who, "up", ld_up, cols)) ||
+        !pitch_ok(who, "q", ld_q, cols))
+        return -1;
+    if (act > LLAMINI_ACT_NONE) { set_error("%s: unknown activation %u", who, act); return -1; }
+    if (rows == 0) return 0;
+    const void* ptrs[] = {d_gate, d_up, d_q, d_scale};
+    if (!d_gate || !d_q || !d_scale) { set_error("%s: null pointer", who); return -1; }
+    if (!align_ok(who, ptrs, 2, act_bytes(type)) || !align_ok(who, ptrs + 3, 1, 4) || !i8_device_ptrs(who, ptrs, 4)) return -1;
+    GluArgs a;
+    a.gate = d_gate; a.up = d_up;
+    a.q = reinterpret_cast<int8_t*>(d_q); a.scale = d_scale;
+    a.ld_gate = ld_gate; a.ld_up = ld_up; a.ld_q = ld_q;
+    a.rows = rows; a.cols = cols; a.act = act;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool ok = type == GGML_TYPE_F32 ? launch_glu<float>(a, st)
+                  : type == GGML_TYPE_F16 ? launch_glu<__half>(a, st) : launch_glu<__nv_bfloat16>(a, st);
+    return ok ? 0 : -1;
+}
