@@ -6,9 +6,17 @@
 // three f32 roundings after them (the sum to f32 and the two scales), the
 // bias's and the output type's are all the rounding there is.
 #include "i8.cuh"
+#include "mma_gemv.cuh"
+#include "pdl.cuh"
+
+#include <atomic>
+#include <cudaTypedefs.h>
 
 namespace lm {
 namespace {
+
+// Set by a kernel whose bounded wait ran out (the outputs of its tile are NaN).
+__device__ uint32_t g_i8_err;
 
 struct GemmI8Args {
     const int8_t* a;
@@ -93,9 +101,377 @@ bool launch_any(const GemmI8Args& g, cudaStream_t st) {
     return LM_CUDA(cudaGetLastError());
 }
 
+// ---------------------------------------------------------------- tensor cores
+
+constexpr uint32_t kSlab = 128;                  // columns (bytes) of both operands in a stage
+constexpr uint64_t kWaitNs = 2000000000ull;      // 2 s
+
+__device__ __forceinline__ uint64_t now_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(t));
+    return t;
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+                 " selp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(bar), "r"(parity), "n"(1000000) : "memory");
+    return done != 0;
+}
+// Waits at most 2 s for the phase of `bar` with this parity; false when the
+// wait ran out, here or in another role of the CTA (*abort).
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort) {
+    const uint32_t b = smem_u32(bar);
+    if (bar_try(b, parity)) return true;
+    const uint64_t t0 = now_ns();
+    for (;;) {
+        if (bar_try(b, parity)) return true;
+        if (*abort) return false;
+        if (now_ns() - t0 > kWaitNs) {
+            *abort = 1u;
+            atomicOr(&g_i8_err, 1u);
+            return false;
+        }
+    }
+}
+// A wait of at most 2 s that an abort does not end: for work already started.
+__device__ __forceinline__ void bar_drain(uint64_t* bar, uint32_t parity) {
+    const uint64_t t0 = now_ns();
+    while (!bar_try(smem_u32(bar), parity) && now_ns() - t0 < kWaitNs) {
+    }
+}
+// Tile of `map` from column x, row y on into this CTA's shared memory.
+__device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
+}
+// Shared-memory descriptor of a K-major operand tile whose rows are 128 bytes
+// in the 128-byte swizzle: 8 rows are 1024 bytes apart from the next 8 (stride
+// byte offset), version 1 (bits 46-47), layout 2 (bits 61-63). 32 columns
+// further is 32 bytes on: the swizzle goes by the address.
+__device__ __forceinline__ uint64_t tile_desc(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// Instruction descriptor of kind::i8: s32 accumulator (bits 4-5 = 2), A and B
+// signed 8-bit (bits 7-9 and 10-12 = 1), both K-major, N >> 3 at bits 17-22, M >> 4
+// at bits 24-28.
+__host__ __device__ constexpr uint32_t i8_idesc(uint32_t M, uint32_t N) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                 " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// One arrival on `bar` once every MMA this thread issued before has finished.
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+                 ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+// 16 columns of this warp's 32 tensor-memory lanes.
+__device__ __forceinline__ void tmem_get16(uint32_t taddr, int* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+                 "tcgen05.wait::ld.sync.aligned;\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t saddr, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(saddr), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ int4 cluster_ld4(uint32_t a) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t cluster_ld(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];\n" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+
+// Up to four neighbouring outputs of one token, from channel n on.
+template <typename T>
+__device__ __forceinline__ void store4(const GemmI8Args& g, uint32_t m, uint32_t n, const float* v, bool vec) {
+    T* o = static_cast<T*>(g.out) + (uint64_t)m * g.ld_out + n;
+    if (vec && n + 4 <= g.n) {
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+            T h[4] = {from_f32<T>(v[0]), from_f32<T>(v[1]), from_f32<T>(v[2]), from_f32<T>(v[3])};
+            *reinterpret_cast<uint2*>(o) = *reinterpret_cast<uint2*>(h);
+        }
+        return;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 4; i++)
+        if (n + i < g.n) o[i] = from_f32<T>(v[i]);
+}
+
+// Few tokens: the weights are what is read, so a tile is 128 channels (the
+// MMA's M: the weights are its A operand, on the tensor memory's lanes) x NT
+// tokens, and a cluster of CTAs splits the columns of a tile so that every SM
+// has a part of the matrix to stream. Warp 4 copies stages of 128 columns of
+// both operands (TMA, 128-byte swizzle), one thread of warp 5 issues the MMAs,
+// warps 0-3 read the sums. The cluster adds its integer sums through distributed
+// shared memory, exact and in any order the same; each CTA finishes a share
+// of the tokens. Nothing is left behind in global memory.
+template <int NT>
+struct Few {
+    static constexpr uint32_t kStage = kSlab * (128 + NT);
+    static constexpr uint32_t kStages = NT == 16 ? 6 : NT == 32 ? 5 : NT == 64 ? 4 : 3;  // two CTAs an SM
+    static constexpr uint32_t kCols = NT < 32 ? 32 : NT;
+    static constexpr size_t kSmem = kStage * kStages + 1024;
+    static_assert(NT * 128 * 4 <= kStage * kStages, "the sums do not fit the stages");
+};
+struct FewShared {
+    uint64_t full[6], empty[6], done;
+    uint32_t tmem, abort;
+};
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(192) gemm_i8_few_kernel(const __grid_constant__ CUtensorMap map_w,
+                                                          const __grid_constant__ CUtensorMap map_a,
+                                                          const GemmI8Args g, uint32_t cs, uint32_t tiles_m) {
+    using F = Few<NT>;
+    extern __shared__ uint8_t sm_raw[];
+    __shared__ FewShared S;
+    const uint32_t base = (smem_u32(sm_raw) + 1023u) & ~1023u;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t rank = cs > 1 ? cluster_rank() : 0u;
+    const uint32_t tile = blockIdx.x / cs;
+    const uint32_t m0 = tile % tiles_m * NT, n0 = tile / tiles_m * 128;
+    const uint32_t nkb = (g.k + kSlab - 1) / kSlab;
+    const uint32_t kb0 = (uint32_t)((uint64_t)nkb * rank / cs), kb1 = (uint32_t)((uint64_t)nkb * (rank + 1) / cs);
+    pdl_trigger();
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < F::kStages; i++) {
+            mbar_init(&S.full[i], 1);
+            mbar_init(&S.empty[i], 1);
+        }
+        mbar_init(&S.done, 1);
+        S.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n"
+                     ::"r"(smem_u32(&S.tmem)), "n"(F::kCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = S.tmem;
+    pdl_wait();
+
+    if (warp == 4) {
+        if (lane == 0) {
+            uint32_t i = 0;
+            for (uint32_t kb = kb0; kb < kb1; kb++, i++) {
+                const uint32_t s = i % F::kStages;
+                if (i >= F::kStages && !bar_wait(&S.empty[s], (i / F::kStages - 1) & 1u, &S.abort)) break;
+                mbar_expect_tx(&S.full[s], F::kStage);
+                tile_load(base + s * F::kStage, &map_w, kb * kSlab, n0, &S.full[s]);
+                tile_load(base + s * F::kStage + 128 * kSlab, &map_a, kb * kSlab, m0, &S.full[s]);
+            }
+            if (i < kb1 - kb0)                       // aborted: let the copies land first
+                for (uint32_t j = i > F::kStages ? i - F::kStages : 0; j < i; j++)
+                    bar_drain(&S.full[j % F::kStages], (j / F::kStages) & 1u);
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {
+            for (uint32_t kb = kb0; kb < kb1; kb++) {
+                const uint32_t i = kb - kb0, s = i % F::kStages;
+                if (!bar_wait(&S.full[s], (i / F::kStages) & 1u, &S.abort)) break;
+                tc_after();
+                const uint32_t steps = min(4u, (g.k - kb * kSlab + 31) / 32);
+                const uint64_t dw = tile_desc(base + s * F::kStage), da = tile_desc(base + s * F::kStage + 128 * kSlab);
+                for (uint32_t j = 0; j < steps; j++)
+                    mma_i8(tmem, dw + 2 * j, da + 2 * j, i8_idesc(128, NT), (i | j) != 0);
+                mma_commit(&S.empty[s]);
+            }
+            mma_commit(&S.done);
+        }
+    }
+    __syncwarp();
+    int* sums = reinterpret_cast<int*>(sm_raw + (base - smem_u32(sm_raw)));     // [NT][128], over the stages
+    const uint32_t mt = min((uint32_t)NT, g.m - m0);
+    const bool vec = (reinterpret_cast<uintptr_t>(g.out) | (g.ld_out * sizeof(T))) % (4 * sizeof(T)) == 0;
+    if (warp < 4) {
+        // every copy has landed and been read once the last MMA has finished
+        if (!bar_wait(&S.done, 0, &S.abort)) bar_drain(&S.done, 0);
+        __syncwarp();
+        tc_after();
+        for (uint32_t c = 0; c < mt; c += 16) {
+            int v[16];
+            tmem_get16(tmem + ((warp * 32u) << 16) + c, v);
+#pragma unroll
+            for (uint32_t i = 0; i < 16; i++)
+                if (kb1 > kb0) sums[(c + i) * 128 + warp * 32 + lane] = v[i];
+                else sums[(c + i) * 128 + warp * 32 + lane] = 0;
+        }
+        tc_before();
+    }
+    __syncthreads();
+    if (cs > 1) cluster_sync();
+    if (warp < 4) {
+        const uint32_t own = smem_u32(sums), ab = smem_u32(&S.abort);
+        const uint32_t n = n0 + 4 * lane;
+        float ws[4], b[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            ws[i] = n + i < g.n ? g.ws[n + i] : 0.f;
+            b[i] = g.bias && n + i < g.n ? g.bias[n + i] : 0.f;
+        }
+        uint32_t bad = 0;
+        for (uint32_t p = 0; p < cs; p++) bad |= cs > 1 ? cluster_ld(cluster_addr(ab, p)) : S.abort;
+        for (uint32_t t = rank * 4 + warp; t < mt; t += 4 * cs) {
+            int4 v = make_int4(0, 0, 0, 0);
+            const uint32_t at = own + (t * 128 + 4 * lane) * 4;
+            if (cs == 1) {
+                v = *reinterpret_cast<const int4*>(sums + t * 128 + 4 * lane);
+            } else {
+                for (uint32_t p = 0; p < cs; p++) {
+                    const int4 x = cluster_ld4(cluster_addr(at, p));
+                    v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+                }
+            }
+            const float as = bad ? NAN : g.as[m0 + t];
+            const int x[4] = {v.x, v.y, v.z, v.w};
+            float y[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                y[i] = (float)x[i] * as * ws[i];
+                if (g.bias) y[i] += b[i];
+            }
+            store4<T>(g, m0 + t, n, y, vec);
+        }
+    }
+    // the others of the cluster may still be reading this CTA's sums
+    __syncwarp();
+    if (cs > 1) cluster_sync();
+    else __syncthreads();
+    if (warp == 5) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "n"(F::kCols) : "memory");
+    }
+}
+
+// cuTensorMapEncodeTiled from the driver, looked up once.
+PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            return (PFN_cuTensorMapEncodeTiled_v12000) nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }();
+    return fn;
+}
+// Tiles of box_rows rows x 128 columns, swizzled; columns and rows past the
+// matrix read as zeros (and zeros add nothing to a sum).
+bool operand_map(CUtensorMap* m, const int8_t* p, uint64_t ld, uint32_t rows, uint32_t cols, uint32_t box_rows) {
+    PFN_cuTensorMapEncodeTiled_v12000 fn = map_encoder();
+    cuuint64_t dims[2] = {cols, rows};
+    cuuint64_t strides[1] = {ld};
+    cuuint32_t box[2] = {kSlab, box_rows}, es[2] = {1, 1};
+    if (fn && fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(p), dims, strides, box, es,
+                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS)
+        return true;
+    set_error("gemm_i8: cuTensorMapEncodeTiled failed");
+    return false;
+}
+
+uint32_t device_sms() {
+    static const uint32_t sms = [] {
+        int dev = 0, n = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess ||
+            cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+            n = 148;
+        return (uint32_t)n;
+    }();
+    return sms;
+}
+
+// Launch with thread-block clusters of `cluster` CTAs and programmatic
+// dependent launch (the kernels wait before their first read of the inputs).
+template <typename... KArgs, typename... Args>
+cudaError_t launch_cluster(void (*kernel)(KArgs...), uint32_t grid, uint32_t block, size_t smem, uint32_t cluster,
+                           cudaStream_t st, Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+// The kernel's limit on dynamic shared memory, raised once a device.
+template <typename K>
+bool allow_smem(std::atomic<uint64_t>& done, K* kernel, size_t bytes) {
+    int dev = 0;
+    if (!LM_CUDA(cudaGetDevice(&dev))) return false;
+    const uint64_t bit = 1ull << (dev & 63);             // (a device past the 63rd sets it at each call)
+    if (dev < 64 && done.load(std::memory_order_acquire) & bit) return true;
+    if (!LM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes))) return false;
+    done.fetch_or(bit, std::memory_order_release);
+    return true;
+}
+
+template <typename T, int NT>
+bool launch_few(const GemmI8Args& g, cudaStream_t st) {
+    using F = Few<NT>;
+    static std::atomic<uint64_t> ready{0};
+    if (!allow_smem(ready, gemm_i8_few_kernel<T, NT>, F::kSmem)) return false;
+    const uint64_t tiles_m = (g.m + NT - 1) / NT, tiles_n = (g.n + 127) / 128, tiles = tiles_m * tiles_n;
+    const uint32_t nkb = (g.k + kSlab - 1) / kSlab;
+    uint32_t cs = 1;
+    while (cs < 8 && tiles * cs * 2 <= 2 * device_sms() && nkb / (cs * 2) >= 2) cs *= 2;
+    if (tiles * cs > 0x7FFFFFFFull) {
+        set_error("gemm_i8: %u x %u outputs are too many for one call", g.m, g.n);
+        return false;
+    }
+    CUtensorMap mw, ma;
+    if (!operand_map(&mw, g.w, g.ld_w, g.n, g.k, 128) || !operand_map(&ma, g.a, g.ld_a, g.m, g.k, NT)) return false;
+    return LM_CUDA(launch_cluster(gemm_i8_few_kernel<T, NT>, (uint32_t)(tiles * cs), 192, F::kSmem, cs, st, mw, ma, g,
+                                  cs, (uint32_t)tiles_m));
+}
+
+// Rows that TMA can read: 16-byte aligned bases and pitches.
+bool tma_rows(const GemmI8Args& g) {
+    return i8_aligned(g.a, 16) && i8_aligned(g.w, 16) && g.ld_a % 16 == 0 && g.ld_w % 16 == 0 &&
+           g.ld_a < (1ull << 40) && g.ld_w < (1ull << 40);
+}
+
 template <typename T>
 bool launch(const GemmI8Args& g, cudaStream_t st) {
-    return launch_any<T>(g, st);
+    if (!tma_rows(g)) return launch_any<T>(g, st);
+    if (g.m <= 16) return launch_few<T, 16>(g, st);
+    if (g.m <= 32) return launch_few<T, 32>(g, st);
+    if (g.m <= 64) return launch_few<T, 64>(g, st);
+    return launch_few<T, 128>(g, st);
 }
 
 }  // namespace
