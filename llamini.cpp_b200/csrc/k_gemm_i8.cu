@@ -10,7 +10,9 @@
 #include "pdl.cuh"
 
 #include <atomic>
+#include <cstdlib>
 #include <cudaTypedefs.h>
+#include <type_traits>
 
 namespace lm {
 namespace {
@@ -118,20 +120,35 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     return done != 0;
 }
 // Waits at most 2 s for the phase of `bar` with this parity; false when the
-// wait ran out, here or in another role of the CTA (*abort).
+// wait ran out, here or in another role of the CTA (*abort). The clock is only
+// looked at after 256 tests: reading it takes some 400 cycles, which a role
+// that waits once a stage would pay once a stage (4096 x 4096 x 11008: 160 us
+// against 105).
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort) {
     const uint32_t b = smem_u32(bar);
-    if (bar_try(b, parity)) return true;
-    const uint64_t t0 = now_ns();
+    uint64_t t0 = 0;
     for (;;) {
-        if (bar_try(b, parity)) return true;
+        for (uint32_t i = 0; i < 256; i++)
+            if (bar_try(b, parity)) return true;
         if (*abort) return false;
-        if (now_ns() - t0 > kWaitNs) {
+        const uint64_t t = now_ns();
+        if (t0 == 0) t0 = t;
+        if (t - t0 > kWaitNs) {
             *abort = 1u;
             atomicOr(&g_i8_err, 1u);
             return false;
         }
     }
+}
+// The same for a wait that is expected to be long: between tests the warp
+// sleeps, since waiting warps that test without a pause slow the MMA and copy
+// warps' own issue (4096 x 4096 x 11008: 190 us against 165).
+__device__ __forceinline__ bool bar_wait_long(uint64_t* bar, uint32_t parity, volatile uint32_t* abort) {
+    for (uint32_t i = 0; i < 4096; i++) {
+        if (bar_try(smem_u32(bar), parity)) return true;
+        __nanosleep(200);
+    }
+    return bar_wait(bar, parity, abort);
 }
 // A wait of at most 2 s that an abort does not end: for work already started.
 __device__ __forceinline__ void bar_drain(uint64_t* bar, uint32_t parity) {
@@ -176,6 +193,15 @@ __device__ __forceinline__ void tmem_get16(uint32_t taddr, int* r) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
                    "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(taddr) : "memory");
+}
+// One lane of a converged warp. The roles' loops are run by whole warps and
+// only the copies and MMAs themselves by the elected lane: operands that are
+// the same in every lane stay in uniform registers, which those instructions
+// read (an MMA every 45 cycles instead of every 125).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
@@ -310,7 +336,7 @@ __global__ void __launch_bounds__(192) gemm_i8_few_kernel(const __grid_constant_
     const bool vec = (reinterpret_cast<uintptr_t>(g.out) | (g.ld_out * sizeof(T))) % (4 * sizeof(T)) == 0;
     if (warp < 4) {
         // every copy has landed and been read once the last MMA has finished
-        if (!bar_wait(&S.done, 0, &S.abort)) bar_drain(&S.done, 0);
+        if (lane == 0 && !bar_wait(&S.done, 0, &S.abort)) bar_drain(&S.done, 0);
         __syncwarp();
         tc_after();
         for (uint32_t c = 0; c < mt; c += 16) {
@@ -368,6 +394,289 @@ __global__ void __launch_bounds__(192) gemm_i8_few_kernel(const __grid_constant_
     }
 }
 
+// Many tokens: a pair of CTAs works on 256 tokens x BN channels at a time, each
+// holding 128 of the tokens' rows and half of the channels' rows in shared
+// memory; one thread of the pair's first CTA issues MMAs that read both
+// (cta_group::2, M = 256) and leave each CTA its 128 tokens' sums in its own
+// tensor memory. Two accumulators alternate, so the epilogue of a tile (four
+// warps: tensor memory -> scales -> shared memory -> TMA store) runs under the
+// next tile's MMAs. Persistent: one pair per two SMs walks the tiles.
+template <typename T, int BN, int SUB>
+struct Many {
+    static constexpr uint32_t kA = SUB * 128 * kSlab, kB = BN / 2 * kSlab, kStage = kA + kB;
+    static constexpr uint32_t kStages = SUB == 2 ? 4 : BN == 256 ? 5 : 7;
+    static constexpr uint32_t kOut = 4096;            // 32 tokens x 128 bytes of outputs
+    static constexpr uint32_t kOuts = SUB == 2 ? 1 : 2;   // of them a warp
+    static constexpr uint32_t kCw = 128 / sizeof(T);
+    static constexpr size_t kSmem = kStage * kStages + 4 * kOuts * kOut + 2 * BN * 4 + 1024;
+    static_assert(kSmem <= 226 * 1024, "shared memory");
+};
+struct ManyShared {
+    uint64_t full[8], empty[8], accf[2], acce[2], done;
+    uint32_t tmem, abort;
+};
+
+__device__ __forceinline__ void bar_arrive_cluster(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_bar) : "memory");
+}
+// As tile_load, the bytes counted on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tile_load_pair(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint32_t cluster_bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];\n"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                 " tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// One arrival on the barrier at this offset of both CTAs.
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
+                 ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void tmem_get32(uint32_t taddr, int* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
+                 " %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+                 "tcgen05.wait::ld.sync.aligned;\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The tile a pair works on at its step: groups of up to 8 token tiles, within
+// a group the token tile changes fastest, so that the tiles in flight share
+// rows of both operands in L2.
+__device__ __forceinline__ void tile_at(uint32_t t, uint32_t tiles_m, uint32_t tiles_n, uint32_t& tm, uint32_t& tn) {
+    const uint32_t per = 8 * tiles_n, grp = t / per, in = t - grp * per, h = min(8u, tiles_m - grp * 8);
+    tm = grp * 8 + in % h;
+    tn = in / h;
+}
+
+template <typename T, int BN, int SUB, bool TMA_OUT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
+    gemm_i8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+                        const __grid_constant__ CUtensorMap map_o, const GemmI8Args g, uint32_t tiles_m, uint32_t tiles_n) {
+    using M = Many<T, BN, SUB>;
+    extern __shared__ uint8_t sm_raw[];
+    __shared__ ManyShared S;
+    const uint32_t base = (smem_u32(sm_raw) + 1023u) & ~1023u;
+    uint8_t* const sm = sm_raw + (base - smem_u32(sm_raw));
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t rank = cluster_rank();
+    const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, tiles = tiles_m * tiles_n;
+    const uint32_t nkb = (g.k + kSlab - 1) / kSlab;
+    pdl_trigger();
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < M::kStages; i++) {
+            mbar_init(&S.full[i], 1);
+            mbar_init(&S.empty[i], 1);
+        }
+        for (uint32_t i = 0; i < 2; i++) {
+            mbar_init(&S.accf[i], 1);
+            mbar_init(&S.acce[i], 8);               // the epilogue warps of both CTAs
+        }
+        mbar_init(&S.done, 1);
+        S.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n"
+                     ::"r"(smem_u32(&S.tmem)), "n"(2 * BN) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();
+    cluster_sync();                                  // both CTAs' barriers exist
+    tc_after();
+    const uint32_t tmem = S.tmem;
+    pdl_wait();
+
+    if (warp == 4) {
+        uint32_t i = 0, s = 0, use = 0;              // stages so far; i = use * kStages + s
+        bool ok = true;
+        for (uint32_t t = pair; t < tiles && ok; t += pairs) {
+            uint32_t tm, tn;
+            tile_at(t, tiles_m, tiles_n, tm, tn);
+            const uint32_t ra = tm * (256 * SUB) + rank * 128, rw = tn * BN + rank * (BN / 2);
+            for (uint32_t kb = 0; kb < nkb; kb++, i++) {
+                if (use && !(ok = bar_wait(&S.empty[s], (use - 1) & 1u, &S.abort))) break;
+                const uint32_t full = cluster_addr(smem_u32(&S.full[s]), 0), at = base + s * M::kStage;
+                if (elect_one()) {
+                    if (rank == 0) mbar_expect_tx(&S.full[s], 2 * M::kStage);
+#pragma unroll
+                    for (uint32_t h = 0; h < SUB; h++)
+                        tile_load_pair(at + h * 128 * kSlab, &map_a, kb * kSlab, ra + h * 256, full);
+                    tile_load_pair(at + M::kA, &map_w, kb * kSlab, rw, full);
+                }
+                __syncwarp();
+                if (++s == M::kStages) {
+                    s = 0;
+                    use++;
+                }
+            }
+        }
+        if (!ok && rank == 0 && lane == 0)           // aborted: let the copies land first
+            for (uint32_t j = i > M::kStages ? i - M::kStages : 0; j < i; j++)
+                bar_drain(&S.full[j % M::kStages], (j / M::kStages) & 1u);
+    } else if (warp == 5) {
+        if (rank == 0) {
+            uint32_t s = 0, use = 0, it = 0;         // it: tiles, of SUB accumulators each
+            bool ok = true;
+            for (uint32_t t = pair; t < tiles && ok; t += pairs, it++) {
+#pragma unroll
+                for (uint32_t h = 0; h < SUB; h++) {
+                    const uint32_t acc = it * SUB + h;
+                    if (acc >= 2 && ok) ok = bar_wait(&S.acce[acc & 1u], (acc / 2 - 1) & 1u, &S.abort);
+                }
+                for (uint32_t kb = 0; kb < nkb && ok; kb++) {
+                    if (!(ok = bar_wait(&S.full[s], use & 1u, &S.abort))) break;
+                    tc_after();
+                    if (elect_one()) {
+                        const uint64_t dw = tile_desc(base + s * M::kStage + M::kA);
+                        const uint32_t steps = (g.k - kb * kSlab + 31) / 32;
+#pragma unroll
+                        for (uint32_t h = 0; h < SUB; h++) {
+                            const uint64_t da = tile_desc(base + s * M::kStage + h * 128 * kSlab);
+                            const uint32_t d = tmem + ((it * SUB + h) & 1u) * BN;
+#pragma unroll
+                            for (uint32_t j = 0; j < 4; j++)
+                                if (j < steps) mma_i8_pair(d, da + 2 * j, dw + 2 * j, i8_idesc(256, BN), (kb | j) != 0);
+                        }
+                        mma_commit_pair(&S.empty[s]);
+                        if (kb + 1 == nkb)
+                            for (uint32_t h = 0; h < SUB; h++) mma_commit_pair(&S.accf[(it * SUB + h) & 1u]);
+                    }
+                    __syncwarp();
+                    if (++s == M::kStages) {
+                        s = 0;
+                        use++;
+                    }
+                }
+            }
+            if (elect_one()) mma_commit_pair(&S.done);
+        }
+    } else if (warp < 4) {
+        float* const sw = reinterpret_cast<float*>(sm + M::kStage * M::kStages + 4 * M::kOuts * M::kOut);
+        float* const sb = sw + BN;
+        uint8_t* const out = sm + M::kStage * M::kStages + warp * M::kOuts * M::kOut;
+        const uint32_t out_a = smem_u32(out);
+        uint32_t it = 0, nst = 0;
+        bool bad = false;
+        for (uint32_t t = pair; t < tiles; t += pairs, it++) {
+            uint32_t tm, tn;
+            tile_at(t, tiles_m, tiles_n, tm, tn);
+            const uint32_t n0 = tn * BN;
+            asm volatile("bar.sync 1, 128;\n" ::: "memory");      // the tile before has read its scales
+            for (uint32_t i = threadIdx.x; i < BN; i += 128) {
+                sw[i] = n0 + i < g.n ? g.ws[n0 + i] : 0.f;
+                sb[i] = g.bias && n0 + i < g.n ? g.bias[n0 + i] : 0.f;
+            }
+            asm volatile("bar.sync 1, 128;\n" ::: "memory");
+#pragma unroll 1
+            for (uint32_t half = 0; half < SUB; half++) {
+            const uint32_t acc = it * SUB + half, buf = acc & 1u, r0 = (tm * SUB + half) * 256 + rank * 128 + warp * 32;
+            const float as = r0 + lane < g.m ? g.as[r0 + lane] : 0.f;
+            bad |= !bar_wait_long(&S.accf[buf], (acc / 2) & 1u, &S.abort);
+            bad = __any_sync(0xffffffffu, bad);
+            tc_after();
+            const uint32_t chunks = min((uint32_t)(BN / M::kCw), (g.n - n0 + M::kCw - 1) / M::kCw);
+            for (uint32_t c = 0; c < chunks; c++, nst++) {
+                uint8_t* const o = out + (nst % M::kOuts) * M::kOut + lane * 128;
+                if (TMA_OUT) {                       // the store before the last from this buffer has read it
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(M::kOuts - 1) : "memory");
+                }
+                __syncwarp();
+#pragma unroll
+                for (uint32_t h = 0; h < M::kCw / 32; h++) {
+                    int v[32];
+                    const uint32_t col = c * M::kCw + h * 32;
+                    tmem_get32(tmem + ((warp * 32u) << 16) + buf * BN + col, v);
+                    float y[32];
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; i += 4) {
+                        const float4 w4 = *reinterpret_cast<const float4*>(sw + col + i);
+                        y[i] = (float)v[i] * as * w4.x;
+                        y[i + 1] = (float)v[i + 1] * as * w4.y;
+                        y[i + 2] = (float)v[i + 2] * as * w4.z;
+                        y[i + 3] = (float)v[i + 3] * as * w4.w;
+                        if (g.bias) {
+                            const float4 b4 = *reinterpret_cast<const float4*>(sb + col + i);
+                            y[i] += b4.x; y[i + 1] += b4.y; y[i + 2] += b4.z; y[i + 3] += b4.w;
+                        }
+                    }
+                    if (bad)
+                        for (uint32_t i = 0; i < 32; i++) y[i] = NAN;
+                    // 16-byte unit u of a token's 128 bytes lies at u ^ (token % 8)
+                    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                        for (uint32_t u = 0; u < 8; u++)
+                            *reinterpret_cast<float4*>(o + ((u ^ (lane & 7u)) << 4)) =
+                                make_float4(y[4 * u], y[4 * u + 1], y[4 * u + 2], y[4 * u + 3]);
+                    } else {
+#pragma unroll
+                        for (uint32_t u = 0; u < 4; u++) {
+                            uint4 p;
+                            p.x = pack2(y[8 * u], y[8 * u + 1], T());
+                            p.y = pack2(y[8 * u + 2], y[8 * u + 3], T());
+                            p.z = pack2(y[8 * u + 4], y[8 * u + 5], T());
+                            p.w = pack2(y[8 * u + 6], y[8 * u + 7], T());
+                            *reinterpret_cast<uint4*>(o + (((h * 4 + u) ^ (lane & 7u)) << 4)) = p;
+                        }
+                    }
+                }
+                if (c + 1 == chunks) {               // the accumulator is free for the tile after the next
+                    tc_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive_cluster(cluster_addr(smem_u32(&S.acce[buf]), 0));
+                }
+                if (TMA_OUT) {
+                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (r0 < g.m)
+                            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n"
+                                         ::"l"(reinterpret_cast<uint64_t>(&map_o)), "r"(n0 + c * M::kCw), "r"(r0),
+                                           "r"(out_a + (nst % M::kOuts) * M::kOut) : "memory");
+                        asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+                    }
+                } else {
+                    __syncwarp();
+                    constexpr uint32_t per = 4 / sizeof(T);       // elements of a lane's word
+                    const uint32_t n = n0 + c * M::kCw + lane * per;
+                    for (uint32_t r = 0; r < 32 && r0 + r < g.m; r++) {
+                        const T* word = reinterpret_cast<const T*>(out + (nst % M::kOuts) * M::kOut + r * 128 +
+                                                                   (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4);
+                        T* dst = static_cast<T*>(g.out) + (uint64_t)(r0 + r) * g.ld_out + n;
+#pragma unroll
+                        for (uint32_t e = 0; e < per; e++)
+                            if (n + e < g.n) dst[e] = word[e];
+                    }
+                }
+            }
+            }
+        }
+        if (TMA_OUT && lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
+    }
+    __syncwarp();
+    if (S.abort && threadIdx.x == 0) bar_drain(&S.done, 0);
+    __syncthreads();
+    cluster_sync();                                  // no arrival or MMA of the pair is on its way
+    if (warp == 5) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "n"(2 * BN) : "memory");
+    }
+}
+
 // cuTensorMapEncodeTiled from the driver, looked up once.
 PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
@@ -406,7 +715,8 @@ uint32_t device_sms() {
     return sms;
 }
 
-// Launch with thread-block clusters of `cluster` CTAs and programmatic
+// Launch with thread-block clusters of `cluster` CTAs (0: the kernel's own
+// size) and programmatic
 // dependent launch (the kernels wait before their first read of the inputs).
 template <typename... KArgs, typename... Args>
 cudaError_t launch_cluster(void (*kernel)(KArgs...), uint32_t grid, uint32_t block, size_t smem, uint32_t cluster,
@@ -417,14 +727,19 @@ cudaError_t launch_cluster(void (*kernel)(KArgs...), uint32_t grid, uint32_t blo
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = cluster;
-    at[0].val.clusterDim.y = 1;
-    at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
+    uint32_t n = 0;
+    if (cluster) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = cluster;
+        at[n].val.clusterDim.y = 1;
+        at[n++].val.clusterDim.z = 1;
+    }
+    if (pdl_enabled()) {
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
     cfg.attrs = at;
-    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    cfg.numAttrs = n;
     return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
@@ -459,6 +774,42 @@ bool launch_few(const GemmI8Args& g, cudaStream_t st) {
                                   cs, (uint32_t)tiles_m));
 }
 
+// Outputs in boxes of 32 tokens x 128 bytes, swizzled like the staging buffer.
+bool output_map(CUtensorMap* m, const GemmI8Args& g, CUtensorMapDataType type, uint32_t size) {
+    PFN_cuTensorMapEncodeTiled_v12000 fn = map_encoder();
+    cuuint64_t dims[2] = {g.n, g.m};
+    cuuint64_t strides[1] = {g.ld_out * size};
+    cuuint32_t box[2] = {128 / size, 32}, es[2] = {1, 1};
+    if (fn && fn(m, type, 2, g.out, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                 CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS)
+        return true;
+    set_error("gemm_i8: cuTensorMapEncodeTiled failed");
+    return false;
+}
+template <typename T> constexpr CUtensorMapDataType map_type() {
+    return std::is_same<T, float>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+         : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+template <typename T, int BN, int SUB, bool TMA_OUT>
+bool launch_many(const GemmI8Args& g, cudaStream_t st) {
+    using M = Many<T, BN, SUB>;
+    static std::atomic<uint64_t> ready{0};
+    if (!allow_smem(ready, gemm_i8_many_kernel<T, BN, SUB, TMA_OUT>, M::kSmem)) return false;
+    const uint64_t tiles_m = (g.m + 256 * SUB - 1) / (256 * SUB), tiles_n = (g.n + BN - 1) / BN, pairs = device_sms() / 2;
+    if (tiles_m * tiles_n > 0x7FFFFFFFull) {
+        set_error("gemm_i8: %u x %u outputs are too many for one call", g.m, g.n);
+        return false;
+    }
+    CUtensorMap ma, mw, mo = {};
+    if (!operand_map(&ma, g.a, g.ld_a, g.m, g.k, 128) || !operand_map(&mw, g.w, g.ld_w, g.n, g.k, BN / 2) ||
+        (TMA_OUT && !output_map(&mo, g, map_type<T>(), sizeof(T))))
+        return false;
+    const uint32_t grid = 2 * (uint32_t)(tiles_m * tiles_n < pairs ? tiles_m * tiles_n : pairs);
+    return LM_CUDA(launch_cluster(gemm_i8_many_kernel<T, BN, SUB, TMA_OUT>, grid, 192, M::kSmem, 0, st, ma, mw, mo, g,
+                                  (uint32_t)tiles_m, (uint32_t)tiles_n));
+}
+
 // Rows that TMA can read: 16-byte aligned bases and pitches.
 bool tma_rows(const GemmI8Args& g) {
     return i8_aligned(g.a, 16) && i8_aligned(g.w, 16) && g.ld_a % 16 == 0 && g.ld_w % 16 == 0 &&
@@ -471,6 +822,13 @@ bool launch(const GemmI8Args& g, cudaStream_t st) {
     if (g.m <= 16) return launch_few<T, 16>(g, st);
     if (g.m <= 32) return launch_few<T, 32>(g, st);
     if (g.m <= 64) return launch_few<T, 64>(g, st);
+    static const int exp_bn = getenv("I8_BN") ? atoi(getenv("I8_BN")) : 0;      // TUNING
+    if (exp_bn) {
+        const bool ta = i8_aligned(g.out, 16) && g.ld_out * sizeof(T) % 16 == 0;
+        if (exp_bn == 256) return ta ? launch_many<T, 256, 1, true>(g, st) : launch_many<T, 256, 1, false>(g, st);
+        if (exp_bn == 512) return ta ? launch_many<T, 256, 2, true>(g, st) : launch_many<T, 256, 2, false>(g, st);
+        return ta ? launch_many<T, 128, 1, true>(g, st) : launch_many<T, 128, 1, false>(g, st);
+    }
     return launch_few<T, 128>(g, st);
 }
 
