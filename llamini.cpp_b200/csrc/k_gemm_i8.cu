@@ -146,7 +146,7 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatil
 __device__ __forceinline__ bool bar_wait_long(uint64_t* bar, uint32_t parity, volatile uint32_t* abort) {
     for (uint32_t i = 0; i < 4096; i++) {
         if (bar_try(smem_u32(bar), parity)) return true;
-        __nanosleep(200);
+        __nanosleep(40);
     }
     return bar_wait(bar, parity, abort);
 }
@@ -394,21 +394,22 @@ __global__ void __launch_bounds__(192) gemm_i8_few_kernel(const __grid_constant_
     }
 }
 
-// Many tokens: a pair of CTAs works on 256 tokens x BN channels at a time, each
+// Many tokens: a pair of CTAs works on 256 tokens x 256 channels at a time, each
 // holding 128 of the tokens' rows and half of the channels' rows in shared
 // memory; one thread of the pair's first CTA issues MMAs that read both
 // (cta_group::2, M = 256) and leave each CTA its 128 tokens' sums in its own
-// tensor memory. Two accumulators alternate, so the epilogue of a tile (four
+// tensor memory. Two accumulators alternate, so the epilogue of a tile (eight
 // warps: tensor memory -> scales -> shared memory -> TMA store) runs under the
-// next tile's MMAs. Persistent: one pair per two SMs walks the tiles.
-template <typename T, int BN, int SUB>
+// next tile's MMAs. Persistent: one pair per two SMs walks the tiles. When the
+// last round has work for at most half of the pairs, its tiles are halved to
+// 128 channels, so that more of them share it.
 struct Many {
-    static constexpr uint32_t kA = SUB * 128 * kSlab, kB = BN / 2 * kSlab, kStage = kA + kB;
-    static constexpr uint32_t kStages = SUB == 2 ? 4 : BN == 256 ? 5 : 7;
-    static constexpr uint32_t kOut = 4096;            // 32 tokens x 128 bytes of outputs
-    static constexpr uint32_t kOuts = SUB == 2 ? 1 : 2;   // of them a warp
-    static constexpr uint32_t kCw = 128 / sizeof(T);
-    static constexpr size_t kSmem = kStage * kStages + 4 * kOuts * kOut + 2 * BN * 4 + 1024;
+    static constexpr uint32_t kA = 128 * kSlab, kB = 64 * kSlab, kStage = kA + 2 * kB;
+    static constexpr uint32_t kStages = 5;
+    static constexpr uint32_t kEpi = 8;               // epilogue warps
+    static constexpr uint32_t kOut = 4096;            // 32 tokens x 128 bytes of outputs, one a warp
+    static constexpr uint32_t kThreads = (kEpi + 2) * 32;
+    static constexpr size_t kSmem = kStage * kStages + kEpi * kOut + 2 * 256 * 4 + 1024;
     static_assert(kSmem <= 226 * 1024, "shared memory");
 };
 struct ManyShared {
@@ -453,27 +454,38 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The tile a pair works on at its step: groups of up to 8 token tiles, within
+// The tile a pair works on at step t: groups of up to 8 token tiles, within
 // a group the token tile changes fastest, so that the tiles in flight share
-// rows of both operands in L2.
-__device__ __forceinline__ void tile_at(uint32_t t, uint32_t tiles_m, uint32_t tiles_n, uint32_t& tm, uint32_t& tn) {
-    const uint32_t per = 8 * tiles_n, grp = t / per, in = t - grp * per, h = min(8u, tiles_m - grp * 8);
-    tm = grp * 8 + in % h;
-    tn = in / h;
+// rows of both operands in L2. From step `whole` on, two steps to a tile.
+struct ManyTiles {
+    uint32_t m, n, whole, steps;                     // tiles of tokens and channels; undivided tiles; steps in all
+};
+struct ManyTile {
+    uint32_t tm, n0, bn;                             // token tile, first channel, channels
+};
+__device__ __forceinline__ ManyTile tile_at(uint32_t t, const ManyTiles& T) {
+    uint32_t half = 0;
+    const bool split = t >= T.whole;
+    if (split) {
+        half = (t - T.whole) & 1u;
+        t = T.whole + ((t - T.whole) >> 1);
+    }
+    const uint32_t per = 8 * T.n, grp = t / per, in = t - grp * per, h = min(8u, T.m - grp * 8), tn = in / h;
+    return {grp * 8 + (in - tn * h), tn * 256 + half * 128, split ? 128u : 256u};
 }
 
-template <typename T, int BN, int SUB, bool TMA_OUT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
+template <typename T, bool TMA_OUT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
     gemm_i8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
-                        const __grid_constant__ CUtensorMap map_o, const GemmI8Args g, uint32_t tiles_m, uint32_t tiles_n) {
-    using M = Many<T, BN, SUB>;
+                        const __grid_constant__ CUtensorMap map_o, const GemmI8Args g, const ManyTiles tiles) {
+    using M = Many;
     extern __shared__ uint8_t sm_raw[];
     __shared__ ManyShared S;
     const uint32_t base = (smem_u32(sm_raw) + 1023u) & ~1023u;
     uint8_t* const sm = sm_raw + (base - smem_u32(sm_raw));
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     const uint32_t rank = cluster_rank();
-    const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, tiles = tiles_m * tiles_n;
+    const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const uint32_t nkb = (g.k + kSlab - 1) / kSlab;
     pdl_trigger();
     if (threadIdx.x == 0) {
@@ -483,15 +495,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
         }
         for (uint32_t i = 0; i < 2; i++) {
             mbar_init(&S.accf[i], 1);
-            mbar_init(&S.acce[i], 8);               // the epilogue warps of both CTAs
+            mbar_init(&S.acce[i], 2 * M::kEpi);      // the epilogue warps of both CTAs
         }
         mbar_init(&S.done, 1);
         S.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    if (warp == 5) {
+    if (warp == M::kEpi + 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n"
-                     ::"r"(smem_u32(&S.tmem)), "n"(2 * BN) : "memory");
+                     ::"r"(smem_u32(&S.tmem)), "n"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
     }
     tc_before();
@@ -501,22 +513,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
     const uint32_t tmem = S.tmem;
     pdl_wait();
 
-    if (warp == 4) {
+    if (warp == M::kEpi) {
         uint32_t i = 0, s = 0, use = 0;              // stages so far; i = use * kStages + s
         bool ok = true;
-        for (uint32_t t = pair; t < tiles && ok; t += pairs) {
-            uint32_t tm, tn;
-            tile_at(t, tiles_m, tiles_n, tm, tn);
-            const uint32_t ra = tm * (256 * SUB) + rank * 128, rw = tn * BN + rank * (BN / 2);
+        for (uint32_t t = pair; t < tiles.steps && ok; t += pairs) {
+            const ManyTile q = tile_at(t, tiles);
+            if (q.n0 >= g.n) continue;               // the empty second half of a last tile
+            const uint32_t ra = q.tm * 256 + rank * 128, rw = q.n0 + rank * (q.bn / 2);
+            const bool whole = q.bn == 256;
             for (uint32_t kb = 0; kb < nkb; kb++, i++) {
                 if (use && !(ok = bar_wait(&S.empty[s], (use - 1) & 1u, &S.abort))) break;
                 const uint32_t full = cluster_addr(smem_u32(&S.full[s]), 0), at = base + s * M::kStage;
                 if (elect_one()) {
-                    if (rank == 0) mbar_expect_tx(&S.full[s], 2 * M::kStage);
-#pragma unroll
-                    for (uint32_t h = 0; h < SUB; h++)
-                        tile_load_pair(at + h * 128 * kSlab, &map_a, kb * kSlab, ra + h * 256, full);
+                    if (rank == 0) mbar_expect_tx(&S.full[s], 2 * (M::kA + (whole ? 2 : 1) * M::kB));
+                    tile_load_pair(at, &map_a, kb * kSlab, ra, full);
                     tile_load_pair(at + M::kA, &map_w, kb * kSlab, rw, full);
+                    if (whole) tile_load_pair(at + M::kA + M::kB, &map_w, kb * kSlab, rw + 64, full);
                 }
                 __syncwarp();
                 if (++s == M::kStages) {
@@ -528,33 +540,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
         if (!ok && rank == 0 && lane == 0)           // aborted: let the copies land first
             for (uint32_t j = i > M::kStages ? i - M::kStages : 0; j < i; j++)
                 bar_drain(&S.full[j % M::kStages], (j / M::kStages) & 1u);
-    } else if (warp == 5) {
+    } else if (warp == M::kEpi + 1) {
         if (rank == 0) {
-            uint32_t s = 0, use = 0, it = 0;         // it: tiles, of SUB accumulators each
+            uint32_t s = 0, use = 0, acc = 0;
             bool ok = true;
-            for (uint32_t t = pair; t < tiles && ok; t += pairs, it++) {
-#pragma unroll
-                for (uint32_t h = 0; h < SUB; h++) {
-                    const uint32_t acc = it * SUB + h;
-                    if (acc >= 2 && ok) ok = bar_wait(&S.acce[acc & 1u], (acc / 2 - 1) & 1u, &S.abort);
-                }
-                for (uint32_t kb = 0; kb < nkb && ok; kb++) {
+            for (uint32_t t = pair; t < tiles.steps && ok; t += pairs) {
+                const ManyTile q = tile_at(t, tiles);
+                if (q.n0 >= g.n) continue;
+                const uint32_t buf = acc & 1u, d = tmem + buf * 256;
+                const uint32_t idesc = q.bn == 256 ? i8_idesc(256, 256) : i8_idesc(256, 128);
+                if (acc >= 2 && !(ok = bar_wait(&S.acce[buf], (acc / 2 - 1) & 1u, &S.abort))) break;
+                for (uint32_t kb = 0; kb < nkb; kb++) {
                     if (!(ok = bar_wait(&S.full[s], use & 1u, &S.abort))) break;
                     tc_after();
                     if (elect_one()) {
-                        const uint64_t dw = tile_desc(base + s * M::kStage + M::kA);
+                        const uint64_t da = tile_desc(base + s * M::kStage), dw = tile_desc(base + s * M::kStage + M::kA);
                         const uint32_t steps = (g.k - kb * kSlab + 31) / 32;
 #pragma unroll
-                        for (uint32_t h = 0; h < SUB; h++) {
-                            const uint64_t da = tile_desc(base + s * M::kStage + h * 128 * kSlab);
-                            const uint32_t d = tmem + ((it * SUB + h) & 1u) * BN;
-#pragma unroll
-                            for (uint32_t j = 0; j < 4; j++)
-                                if (j < steps) mma_i8_pair(d, da + 2 * j, dw + 2 * j, i8_idesc(256, BN), (kb | j) != 0);
-                        }
+                        for (uint32_t j = 0; j < 4; j++)
+                            if (j < steps) mma_i8_pair(d, da + 2 * j, dw + 2 * j, idesc, (kb | j) != 0);
                         mma_commit_pair(&S.empty[s]);
-                        if (kb + 1 == nkb)
-                            for (uint32_t h = 0; h < SUB; h++) mma_commit_pair(&S.accf[(it * SUB + h) & 1u]);
+                        if (kb + 1 == nkb) mma_commit_pair(&S.accf[buf]);
                     }
                     __syncwarp();
                     if (++s == M::kStages) {
@@ -562,100 +568,105 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
                         use++;
                     }
                 }
+                acc++;
             }
             if (elect_one()) mma_commit_pair(&S.done);
         }
-    } else if (warp < 4) {
-        float* const sw = reinterpret_cast<float*>(sm + M::kStage * M::kStages + 4 * M::kOuts * M::kOut);
-        float* const sb = sw + BN;
-        uint8_t* const out = sm + M::kStage * M::kStages + warp * M::kOuts * M::kOut;
-        const uint32_t out_a = smem_u32(out);
-        uint32_t it = 0, nst = 0;
+    } else {
+        constexpr uint32_t kCw = 128 / sizeof(T);    // channels of a staged chunk
+        const uint32_t quad = warp & 3u, side = warp >> 2;   // tensor-memory lanes; half of the tile's channels
+        float* const sw = reinterpret_cast<float*>(sm + M::kStage * M::kStages + M::kEpi * M::kOut);
+        float* const sb = sw + 256;
+        uint8_t* const out = sm + M::kStage * M::kStages + warp * M::kOut;
+        uint32_t acc = 0;
         bool bad = false;
-        for (uint32_t t = pair; t < tiles; t += pairs, it++) {
-            uint32_t tm, tn;
-            tile_at(t, tiles_m, tiles_n, tm, tn);
-            const uint32_t n0 = tn * BN;
-            asm volatile("bar.sync 1, 128;\n" ::: "memory");      // the tile before has read its scales
-            for (uint32_t i = threadIdx.x; i < BN; i += 128) {
-                sw[i] = n0 + i < g.n ? g.ws[n0 + i] : 0.f;
-                sb[i] = g.bias && n0 + i < g.n ? g.bias[n0 + i] : 0.f;
-            }
-            asm volatile("bar.sync 1, 128;\n" ::: "memory");
-#pragma unroll 1
-            for (uint32_t half = 0; half < SUB; half++) {
-            const uint32_t acc = it * SUB + half, buf = acc & 1u, r0 = (tm * SUB + half) * 256 + rank * 128 + warp * 32;
-            const float as = r0 + lane < g.m ? g.as[r0 + lane] : 0.f;
+        // the scales of a tile are loaded while the tile before is finished
+        float ws_next = 0.f, b_next = 0.f, as_next = 0.f;
+        auto load_scales = [&](uint32_t t) {
+            if (t >= tiles.steps) return;
+            const ManyTile q = tile_at(t, tiles);
+            const uint32_t n = q.n0 + threadIdx.x, r = q.tm * 256 + rank * 128 + quad * 32 + lane;
+            ws_next = n < g.n ? g.ws[n] : 0.f;
+            b_next = g.bias && n < g.n ? g.bias[n] : 0.f;
+            as_next = r < g.m ? g.as[r] : 0.f;
+        };
+        load_scales(pair);
+        for (uint32_t t = pair; t < tiles.steps; t += pairs) {
+            const ManyTile q = tile_at(t, tiles);
+            if (q.n0 >= g.n) break;                  // (only ever the last step)
+            const uint32_t buf = acc & 1u, r0 = q.tm * 256 + rank * 128 + quad * 32;
+            asm volatile("bar.sync 1, 256;\n" ::: "memory");      // the tile before has read its scales
+            sw[threadIdx.x] = ws_next;
+            sb[threadIdx.x] = b_next;
+            const float as = as_next;
+            load_scales(t + pairs);
+            asm volatile("bar.sync 1, 256;\n" ::: "memory");
             bad |= !bar_wait_long(&S.accf[buf], (acc / 2) & 1u, &S.abort);
             bad = __any_sync(0xffffffffu, bad);
             tc_after();
-            const uint32_t chunks = min((uint32_t)(BN / M::kCw), (g.n - n0 + M::kCw - 1) / M::kCw);
-            for (uint32_t c = 0; c < chunks; c++, nst++) {
-                uint8_t* const o = out + (nst % M::kOuts) * M::kOut + lane * 128;
-                if (TMA_OUT) {                       // the store before the last from this buffer has read it
-                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(M::kOuts - 1) : "memory");
-                }
-                __syncwarp();
+            const uint32_t c0 = side * (q.bn / 2), left = g.n - q.n0;
+            const uint32_t c1 = min(c0 + q.bn / 2, left);
+            for (uint32_t c = c0; c < c1; c += kCw) {
+                uint4 p[8];                          // this token's 128 bytes
 #pragma unroll
-                for (uint32_t h = 0; h < M::kCw / 32; h++) {
+                for (uint32_t h = 0; h < kCw / 32; h++) {
                     int v[32];
-                    const uint32_t col = c * M::kCw + h * 32;
-                    tmem_get32(tmem + ((warp * 32u) << 16) + buf * BN + col, v);
+                    tmem_get32(tmem + ((quad * 32u) << 16) + buf * 256 + c + h * 32, v);
                     float y[32];
 #pragma unroll
                     for (uint32_t i = 0; i < 32; i += 4) {
-                        const float4 w4 = *reinterpret_cast<const float4*>(sw + col + i);
+                        const float4 w4 = *reinterpret_cast<const float4*>(sw + c + h * 32 + i);
                         y[i] = (float)v[i] * as * w4.x;
                         y[i + 1] = (float)v[i + 1] * as * w4.y;
                         y[i + 2] = (float)v[i + 2] * as * w4.z;
                         y[i + 3] = (float)v[i + 3] * as * w4.w;
-                        if (g.bias) {
-                            const float4 b4 = *reinterpret_cast<const float4*>(sb + col + i);
+                    }
+                    if (g.bias) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 32; i += 4) {
+                            const float4 b4 = *reinterpret_cast<const float4*>(sb + c + h * 32 + i);
                             y[i] += b4.x; y[i + 1] += b4.y; y[i + 2] += b4.z; y[i + 3] += b4.w;
                         }
                     }
-                    if (bad)
+                    if (bad) {
+#pragma unroll
                         for (uint32_t i = 0; i < 32; i++) y[i] = NAN;
-                    // 16-byte unit u of a token's 128 bytes lies at u ^ (token % 8)
+                    }
                     if constexpr (sizeof(T) == 4) {
 #pragma unroll
                         for (uint32_t u = 0; u < 8; u++)
-                            *reinterpret_cast<float4*>(o + ((u ^ (lane & 7u)) << 4)) =
-                                make_float4(y[4 * u], y[4 * u + 1], y[4 * u + 2], y[4 * u + 3]);
+                            p[u] = make_uint4(__float_as_uint(y[4 * u]), __float_as_uint(y[4 * u + 1]),
+                                              __float_as_uint(y[4 * u + 2]), __float_as_uint(y[4 * u + 3]));
                     } else {
 #pragma unroll
-                        for (uint32_t u = 0; u < 4; u++) {
-                            uint4 p;
-                            p.x = pack2(y[8 * u], y[8 * u + 1], T());
-                            p.y = pack2(y[8 * u + 2], y[8 * u + 3], T());
-                            p.z = pack2(y[8 * u + 4], y[8 * u + 5], T());
-                            p.w = pack2(y[8 * u + 6], y[8 * u + 7], T());
-                            *reinterpret_cast<uint4*>(o + (((h * 4 + u) ^ (lane & 7u)) << 4)) = p;
-                        }
+                        for (uint32_t u = 0; u < 4; u++)
+                            p[h * 4 + u] = make_uint4(pack2(y[8 * u], y[8 * u + 1], T()), pack2(y[8 * u + 2], y[8 * u + 3], T()),
+                                                      pack2(y[8 * u + 4], y[8 * u + 5], T()), pack2(y[8 * u + 6], y[8 * u + 7], T()));
                     }
                 }
-                if (c + 1 == chunks) {               // the accumulator is free for the tile after the next
-                    tc_before();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive_cluster(cluster_addr(smem_u32(&S.acce[buf]), 0));
-                }
+                if (TMA_OUT && lane == 0)            // the store before has read the buffer
+                    asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
+                __syncwarp();
+                // 16-byte unit u of a token's 128 bytes lies at u ^ (token % 8)
+#pragma unroll
+                for (uint32_t u = 0; u < 8; u++)
+                    *reinterpret_cast<uint4*>(out + lane * 128 + ((u ^ (lane & 7u)) << 4)) = p[u];
                 if (TMA_OUT) {
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                     __syncwarp();
                     if (lane == 0) {
                         if (r0 < g.m)
                             asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n"
-                                         ::"l"(reinterpret_cast<uint64_t>(&map_o)), "r"(n0 + c * M::kCw), "r"(r0),
-                                           "r"(out_a + (nst % M::kOuts) * M::kOut) : "memory");
+                                         ::"l"(reinterpret_cast<uint64_t>(&map_o)), "r"(q.n0 + c), "r"(r0),
+                                           "r"(smem_u32(out)) : "memory");
                         asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
                     }
                 } else {
                     __syncwarp();
                     constexpr uint32_t per = 4 / sizeof(T);       // elements of a lane's word
-                    const uint32_t n = n0 + c * M::kCw + lane * per;
+                    const uint32_t n = q.n0 + c + lane * per;
                     for (uint32_t r = 0; r < 32 && r0 + r < g.m; r++) {
-                        const T* word = reinterpret_cast<const T*>(out + (nst % M::kOuts) * M::kOut + r * 128 +
-                                                                   (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4);
+                        const T* word = reinterpret_cast<const T*>(out + r * 128 + (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4);
                         T* dst = static_cast<T*>(g.out) + (uint64_t)(r0 + r) * g.ld_out + n;
 #pragma unroll
                         for (uint32_t e = 0; e < per; e++)
@@ -663,7 +674,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
                     }
                 }
             }
-            }
+            // the accumulator is free for the tile after the next
+            tc_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive_cluster(cluster_addr(smem_u32(&S.acce[buf]), 0));
+            acc++;
         }
         if (TMA_OUT && lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
     }
@@ -671,9 +686,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
     if (S.abort && threadIdx.x == 0) bar_drain(&S.done, 0);
     __syncthreads();
     cluster_sync();                                  // no arrival or MMA of the pair is on its way
-    if (warp == 5) {
+    if (warp == M::kEpi + 1) {
         tc_after();
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "n"(2 * BN) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "n"(512) : "memory");
     }
 }
 
@@ -791,23 +806,27 @@ template <typename T> constexpr CUtensorMapDataType map_type() {
          : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 }
 
-template <typename T, int BN, int SUB, bool TMA_OUT>
+template <typename T, bool TMA_OUT>
 bool launch_many(const GemmI8Args& g, cudaStream_t st) {
-    using M = Many<T, BN, SUB>;
     static std::atomic<uint64_t> ready{0};
-    if (!allow_smem(ready, gemm_i8_many_kernel<T, BN, SUB, TMA_OUT>, M::kSmem)) return false;
-    const uint64_t tiles_m = (g.m + 256 * SUB - 1) / (256 * SUB), tiles_n = (g.n + BN - 1) / BN, pairs = device_sms() / 2;
-    if (tiles_m * tiles_n > 0x7FFFFFFFull) {
+    if (!allow_smem(ready, gemm_i8_many_kernel<T, TMA_OUT>, Many::kSmem)) return false;
+    const uint64_t tm = (g.m + 255) / 256, tn = (g.n + 255) / 256, n = tm * tn, pairs = device_sms() / 2;
+    if (n > 0x3FFFFFFFull) {
         set_error("gemm_i8: %u x %u outputs are too many for one call", g.m, g.n);
         return false;
     }
+    const uint64_t rest = n % pairs, split = 2 * rest <= pairs ? rest : 0;
+    const ManyTiles tiles = {(uint32_t)tm, (uint32_t)tn, (uint32_t)(n - split), (uint32_t)(n + split)};
     CUtensorMap ma, mw, mo = {};
-    if (!operand_map(&ma, g.a, g.ld_a, g.m, g.k, 128) || !operand_map(&mw, g.w, g.ld_w, g.n, g.k, BN / 2) ||
+    if (!operand_map(&ma, g.a, g.ld_a, g.m, g.k, 128) || !operand_map(&mw, g.w, g.ld_w, g.n, g.k, 64) ||
         (TMA_OUT && !output_map(&mo, g, map_type<T>(), sizeof(T))))
         return false;
-    const uint32_t grid = 2 * (uint32_t)(tiles_m * tiles_n < pairs ? tiles_m * tiles_n : pairs);
-    return LM_CUDA(launch_cluster(gemm_i8_many_kernel<T, BN, SUB, TMA_OUT>, grid, 192, M::kSmem, 0, st, ma, mw, mo, g,
-                                  (uint32_t)tiles_m, (uint32_t)tiles_n));
+    const uint32_t grid = 2 * (uint32_t)(tiles.steps < pairs ? tiles.steps : pairs);
+    return LM_CUDA(launch_cluster(gemm_i8_many_kernel<T, TMA_OUT>, grid, Many::kThreads, Many::kSmem, 0, st, ma, mw, mo, g, tiles));
+}
+template <typename T>
+bool launch_many(const GemmI8Args& g, cudaStream_t st) {
+    return i8_aligned(g.out, 16) && g.ld_out * sizeof(T) % 16 == 0 ? launch_many<T, true>(g, st) : launch_many<T, false>(g, st);
 }
 
 // Rows that TMA can read: 16-byte aligned bases and pitches.
@@ -823,12 +842,7 @@ bool launch(const GemmI8Args& g, cudaStream_t st) {
     if (g.m <= 32) return launch_few<T, 32>(g, st);
     if (g.m <= 64) return launch_few<T, 64>(g, st);
     static const int exp_bn = getenv("I8_BN") ? atoi(getenv("I8_BN")) : 0;      // TUNING
-    if (exp_bn) {
-        const bool ta = i8_aligned(g.out, 16) && g.ld_out * sizeof(T) % 16 == 0;
-        if (exp_bn == 256) return ta ? launch_many<T, 256, 1, true>(g, st) : launch_many<T, 256, 1, false>(g, st);
-        if (exp_bn == 512) return ta ? launch_many<T, 256, 2, true>(g, st) : launch_many<T, 256, 2, false>(g, st);
-        return ta ? launch_many<T, 128, 1, true>(g, st) : launch_many<T, 128, 1, false>(g, st);
-    }
+    if (exp_bn) return launch_many<T>(g, st);
     return launch_few<T, 128>(g, st);
 }
 
