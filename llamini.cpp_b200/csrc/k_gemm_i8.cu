@@ -10,7 +10,6 @@
 #include "pdl.cuh"
 
 #include <atomic>
-#include <cstdlib>
 #include <cudaTypedefs.h>
 #include <type_traits>
 
@@ -248,9 +247,9 @@ __device__ __forceinline__ void store4(const GemmI8Args& g, uint32_t m, uint32_t
 // Few tokens: the weights are what is read, so a tile is 128 channels (the
 // MMA's M: the weights are its A operand, on the tensor memory's lanes) x NT
 // tokens, and a cluster of CTAs splits the columns of a tile so that every SM
-// has a part of the matrix to stream. Warp 4 copies stages of 128 columns of
-// both operands (TMA, 128-byte swizzle), one thread of warp 5 issues the MMAs,
-// warps 0-3 read the sums. The cluster adds its integer sums through distributed
+// has a part of the matrix to stream. Warp 8 copies stages of 128 columns of
+// both operands (TMA, 128-byte swizzle), one thread of warp 9 issues the MMAs,
+// warps 0-7 read the sums. The cluster adds its integer sums through distributed
 // shared memory, exact and in any order the same; each CTA finishes a share
 // of the tokens. Nothing is left behind in global memory.
 template <int NT>
@@ -258,16 +257,19 @@ struct Few {
     static constexpr uint32_t kStage = kSlab * (128 + NT);
     static constexpr uint32_t kStages = NT == 16 ? 6 : NT == 32 ? 5 : NT == 64 ? 4 : 3;  // two CTAs an SM
     static constexpr uint32_t kCols = NT < 32 ? 32 : NT;
+    static constexpr uint32_t kEpi = 8;              // epilogue warps
+    static constexpr uint32_t kThreads = (kEpi + 2) * 32;
     static constexpr size_t kSmem = kStage * kStages + 1024;
     static_assert(NT * 128 * 4 <= kStage * kStages, "the sums do not fit the stages");
 };
 struct FewShared {
     uint64_t full[6], empty[6], done;
     uint32_t tmem, abort;
+    float as[128];
 };
 
 template <typename T, int NT>
-__global__ void __launch_bounds__(192) gemm_i8_few_kernel(const __grid_constant__ CUtensorMap map_w,
+__global__ void __launch_bounds__(Few<NT>::kThreads, 2) gemm_i8_few_kernel(const __grid_constant__ CUtensorMap map_w,
                                                           const __grid_constant__ CUtensorMap map_a,
                                                           const GemmI8Args g, uint32_t cs, uint32_t tiles_m) {
     using F = Few<NT>;
@@ -290,7 +292,7 @@ __global__ void __launch_bounds__(192) gemm_i8_few_kernel(const __grid_constant_
         S.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    if (warp == 5) {
+    if (warp == F::kEpi + 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n"
                      ::"r"(smem_u32(&S.tmem)), "n"(F::kCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
@@ -301,79 +303,81 @@ __global__ void __launch_bounds__(192) gemm_i8_few_kernel(const __grid_constant_
     const uint32_t tmem = S.tmem;
     pdl_wait();
 
-    if (warp == 4) {
-        if (lane == 0) {
-            uint32_t i = 0;
-            for (uint32_t kb = kb0; kb < kb1; kb++, i++) {
-                const uint32_t s = i % F::kStages;
-                if (i >= F::kStages && !bar_wait(&S.empty[s], (i / F::kStages - 1) & 1u, &S.abort)) break;
+    if (warp == F::kEpi) {
+        uint32_t i = 0, s = 0, use = 0;              // stages so far; i = use * kStages + s
+        for (uint32_t kb = kb0; kb < kb1; kb++, i++) {
+            if (use && !bar_wait(&S.empty[s], (use - 1) & 1u, &S.abort)) break;
+            if (elect_one()) {
                 mbar_expect_tx(&S.full[s], F::kStage);
                 tile_load(base + s * F::kStage, &map_w, kb * kSlab, n0, &S.full[s]);
                 tile_load(base + s * F::kStage + 128 * kSlab, &map_a, kb * kSlab, m0, &S.full[s]);
             }
-            if (i < kb1 - kb0)                       // aborted: let the copies land first
-                for (uint32_t j = i > F::kStages ? i - F::kStages : 0; j < i; j++)
-                    bar_drain(&S.full[j % F::kStages], (j / F::kStages) & 1u);
+            __syncwarp();
+            if (++s == F::kStages) {
+                s = 0;
+                use++;
+            }
         }
-    } else if (warp == 5) {
-        if (lane == 0) {
-            for (uint32_t kb = kb0; kb < kb1; kb++) {
-                const uint32_t i = kb - kb0, s = i % F::kStages;
-                if (!bar_wait(&S.full[s], (i / F::kStages) & 1u, &S.abort)) break;
-                tc_after();
-                const uint32_t steps = min(4u, (g.k - kb * kSlab + 31) / 32);
+        if (i < kb1 - kb0 && lane == 0)              // aborted: let the copies land first
+            for (uint32_t j = i > F::kStages ? i - F::kStages : 0; j < i; j++)
+                bar_drain(&S.full[j % F::kStages], (j / F::kStages) & 1u);
+    } else if (warp == F::kEpi + 1) {
+        uint32_t s = 0, use = 0;
+        for (uint32_t kb = kb0; kb < kb1; kb++) {
+            if (!bar_wait(&S.full[s], use & 1u, &S.abort)) break;
+            tc_after();
+            if (elect_one()) {
+                const uint32_t steps = (g.k - kb * kSlab + 31) / 32;
                 const uint64_t dw = tile_desc(base + s * F::kStage), da = tile_desc(base + s * F::kStage + 128 * kSlab);
-                for (uint32_t j = 0; j < steps; j++)
-                    mma_i8(tmem, dw + 2 * j, da + 2 * j, i8_idesc(128, NT), (i | j) != 0);
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++)
+                    if (j < steps) mma_i8(tmem, dw + 2 * j, da + 2 * j, i8_idesc(128, NT), ((kb - kb0) | j) != 0);
                 mma_commit(&S.empty[s]);
             }
-            mma_commit(&S.done);
+            __syncwarp();
+            if (++s == F::kStages) {
+                s = 0;
+                use++;
+            }
         }
+        if (elect_one()) mma_commit(&S.done);
     }
     __syncwarp();
     int* sums = reinterpret_cast<int*>(sm_raw + (base - smem_u32(sm_raw)));     // [NT][128], over the stages
-    const uint32_t mt = min((uint32_t)NT, g.m - m0);
-    const bool vec = (reinterpret_cast<uintptr_t>(g.out) | (g.ld_out * sizeof(T))) % (4 * sizeof(T)) == 0;
-    if (warp < 4) {
-        // every copy has landed and been read once the last MMA has finished
-        if (lane == 0 && !bar_wait(&S.done, 0, &S.abort)) bar_drain(&S.done, 0);
-        __syncwarp();
-        tc_after();
-        for (uint32_t c = 0; c < mt; c += 16) {
-            int v[16];
-            tmem_get16(tmem + ((warp * 32u) << 16) + c, v);
-#pragma unroll
-            for (uint32_t i = 0; i < 16; i++)
-                if (kb1 > kb0) sums[(c + i) * 128 + warp * 32 + lane] = v[i];
-                else sums[(c + i) * 128 + warp * 32 + lane] = 0;
-        }
-        tc_before();
-    }
-    __syncthreads();
-    if (cs > 1) cluster_sync();
-    if (warp < 4) {
-        const uint32_t own = smem_u32(sums), ab = smem_u32(&S.abort);
-        const uint32_t n = n0 + 4 * lane;
-        float ws[4], b[4];
+    const uint32_t mt = min((uint32_t)NT, g.m - m0), n = n0 + 4 * lane;
+    float ws[4], b[4];                               // this lane's four channels
+    if (warp < F::kEpi) {
 #pragma unroll
         for (uint32_t i = 0; i < 4; i++) {
             ws[i] = n + i < g.n ? g.ws[n + i] : 0.f;
             b[i] = g.bias && n + i < g.n ? g.bias[n + i] : 0.f;
         }
-        uint32_t bad = 0;
-        for (uint32_t p = 0; p < cs; p++) bad |= cs > 1 ? cluster_ld(cluster_addr(ab, p)) : S.abort;
-        for (uint32_t t = rank * 4 + warp; t < mt; t += 4 * cs) {
-            int4 v = make_int4(0, 0, 0, 0);
-            const uint32_t at = own + (t * 128 + 4 * lane) * 4;
-            if (cs == 1) {
-                v = *reinterpret_cast<const int4*>(sums + t * 128 + 4 * lane);
-            } else {
-                for (uint32_t p = 0; p < cs; p++) {
-                    const int4 x = cluster_ld4(cluster_addr(at, p));
-                    v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-                }
-            }
-            const float as = bad ? NAN : g.as[m0 + t];
+        if (threadIdx.x < mt) S.as[threadIdx.x] = g.as[m0 + threadIdx.x];
+        // every copy has landed and been read once the last MMA has finished
+        if (!bar_wait_long(&S.done, 0, &S.abort)) bar_drain(&S.done, 0);
+        __syncwarp();
+        tc_after();
+        for (uint32_t c = (warp >> 2) * 16; c < mt; c += 32) {
+            int v[16];
+            tmem_get16(tmem + (((warp & 3u) * 32u) << 16) + c, v);
+#pragma unroll
+            for (uint32_t i = 0; i < 16; i++) sums[(c + i) * 128 + (warp & 3u) * 32 + lane] = v[i];
+        }
+        tc_before();
+    }
+    __syncthreads();
+    if (cs > 1) cluster_sync();
+    if (warp < F::kEpi) {
+        const bool vec = (reinterpret_cast<uintptr_t>(g.out) | (g.ld_out * sizeof(T))) % (4 * sizeof(T)) == 0;
+        const uint32_t own = smem_u32(sums) + 16 * lane, ab = smem_u32(&S.abort);
+        uint32_t bad = S.abort;
+        if (cs > 1)
+            for (uint32_t p = 0; p < cs; p++) bad |= cluster_ld(cluster_addr(ab, p));
+        // several loads of sums in flight: four tokens at a time, or two
+        // tokens and four CTAs of the cluster
+        const uint32_t step = F::kEpi * cs;
+        auto finish = [&](uint32_t t, const int4& v) {
+            const float as = bad ? NAN : S.as[t];
             const int x[4] = {v.x, v.y, v.z, v.w};
             float y[4];
 #pragma unroll
@@ -382,13 +386,34 @@ __global__ void __launch_bounds__(192) gemm_i8_few_kernel(const __grid_constant_
                 if (g.bias) y[i] += b[i];
             }
             store4<T>(g, m0 + t, n, y, vec);
+        };
+        if (cs == 1) {
+#pragma unroll 4
+            for (uint32_t t = warp; t < mt; t += F::kEpi)
+                finish(t, *reinterpret_cast<const int4*>(sums + t * 128 + 4 * lane));
+        } else {
+            for (uint32_t t = rank * F::kEpi + warp; t < mt; t += 2 * step) {
+                // a second token past the last one reads a row of sums that
+                // exists (NT rows are there) and is not stored
+                const uint32_t t1 = t + step < NT ? t + step : t;
+                int4 v0 = make_int4(0, 0, 0, 0), v1 = v0;
+#pragma unroll 4
+                for (uint32_t p = 0; p < cs; p++) {
+                    const uint32_t at = cluster_addr(own, p);
+                    const int4 x = cluster_ld4(at + t * 512), y = cluster_ld4(at + t1 * 512);
+                    v0.x += x.x; v0.y += x.y; v0.z += x.z; v0.w += x.w;
+                    v1.x += y.x; v1.y += y.y; v1.z += y.z; v1.w += y.w;
+                }
+                finish(t, v0);
+                if (t + step < mt) finish(t + step, v1);
+            }
         }
     }
     // the others of the cluster may still be reading this CTA's sums
     __syncwarp();
     if (cs > 1) cluster_sync();
     else __syncthreads();
-    if (warp == 5) {
+    if (warp == F::kEpi + 1) {
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "n"(F::kCols) : "memory");
     }
@@ -777,6 +802,9 @@ bool launch_few(const GemmI8Args& g, cudaStream_t st) {
     if (!allow_smem(ready, gemm_i8_few_kernel<T, NT>, F::kSmem)) return false;
     const uint64_t tiles_m = (g.m + NT - 1) / NT, tiles_n = (g.n + 127) / 128, tiles = tiles_m * tiles_n;
     const uint32_t nkb = (g.k + kSlab - 1) / kSlab;
+    // as many parts as leave two CTAs an SM and two stages a part (20 tiles of 16
+    // stages: 6.2 us in one part, 4.7 in four or eight; 172 tiles of 32: 21.1 us in
+    // one part, 31.9 in two, which no longer run at once)
     uint32_t cs = 1;
     while (cs < 8 && tiles * cs * 2 <= 2 * device_sms() && nkb / (cs * 2) >= 2) cs *= 2;
     if (tiles * cs > 0x7FFFFFFFull) {
@@ -785,7 +813,7 @@ bool launch_few(const GemmI8Args& g, cudaStream_t st) {
     }
     CUtensorMap mw, ma;
     if (!operand_map(&mw, g.w, g.ld_w, g.n, g.k, 128) || !operand_map(&ma, g.a, g.ld_a, g.m, g.k, NT)) return false;
-    return LM_CUDA(launch_cluster(gemm_i8_few_kernel<T, NT>, (uint32_t)(tiles * cs), 192, F::kSmem, cs, st, mw, ma, g,
+    return LM_CUDA(launch_cluster(gemm_i8_few_kernel<T, NT>, (uint32_t)(tiles * cs), F::kThreads, F::kSmem, cs, st, mw, ma, g,
                                   cs, (uint32_t)tiles_m));
 }
 
@@ -835,15 +863,31 @@ bool tma_rows(const GemmI8Args& g) {
            g.ld_a < (1ull << 40) && g.ld_w < (1ull << 40);
 }
 
+// Which kernel and tile. gemm_i8_few_kernel takes the narrowest token tile (16,
+// 32, 64, 128) that leaves no more than `most` tiles: more tiles are more SMs at
+// work, but each reads its channels' weights again; with long rows fewer tiles
+// and a deeper split of the columns win (64 tokens, 4096 x 4096: 16 wide 9.4 us,
+// 32 wide 8.8, 64 wide 10.3; 128 tokens, 4096 x 11008: 17.5, 15.4 at 64, 17.6 at
+// 128). Past 128 tokens, when even 128-wide tiles are more than that (or the rows
+// too short to split), gemm_i8_many_kernel: 512 tokens x 12288 x 4096 34.5 against 25.5 us, 256 x
+// 32000 x 2048 26.8 against 20.7; 512 x 4096 x 11008 the other way, 26.5 against
+// 28.1. Over 16 shapes x 19 token counts the choice costs 2.5 % on average over
+// the best of all tiles.
 template <typename T>
 bool launch(const GemmI8Args& g, cudaStream_t st) {
     if (!tma_rows(g)) return launch_any<T>(g, st);
-    if (g.m <= 16) return launch_few<T, 16>(g, st);
-    if (g.m <= 32) return launch_few<T, 32>(g, st);
-    if (g.m <= 64) return launch_few<T, 64>(g, st);
-    static const int exp_bn = getenv("I8_BN") ? atoi(getenv("I8_BN")) : 0;      // TUNING
-    if (exp_bn) return launch_many<T>(g, st);
-    return launch_few<T, 128>(g, st);
+    const uint64_t tn = (g.n + 127) / 128, sms = device_sms();
+    const uint32_t nkb = (g.k + kSlab - 1) / kSlab;
+    const uint64_t wide = 6 * sms / 5, most = nkb < 30 ? wide : 3 * sms / 5;
+    uint32_t nt = 16;
+    while (nt < 128 && nt < g.m && (g.m + nt - 1) / nt * tn > most) nt *= 2;
+    if (g.m > 128 && ((g.m + nt - 1) / nt * tn > wide || (nkb <= 16 && nt == 128))) return launch_many<T>(g, st);
+    switch (nt) {
+    case 16: return launch_few<T, 16>(g, st);
+    case 32: return launch_few<T, 32>(g, st);
+    case 64: return launch_few<T, 64>(g, st);
+    default: return launch_few<T, 128>(g, st);
+    }
 }
 
 }  // namespace
