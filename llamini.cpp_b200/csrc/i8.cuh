@@ -15,6 +15,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
+#include <type_traits>
 
 namespace lm {
 
@@ -112,6 +113,139 @@ __device__ __forceinline__ void block_max_sum(uint32_t& m, float& s, uint32_t* r
     for (uint32_t i = 1; i < nw; i++) {
         m = max(m, red[i]);
         s += __uint_as_float(red[32 + i]);
+    }
+}
+
+// ---------------------------------------------------------------- rows in registers
+//
+// A row of 16-byte vectors spread over G threads (a warp, or a whole CTA), V
+// vectors a thread, vector j of thread t at t + j G.
+
+template <typename T> constexpr uint32_t vec_elems() { return 16 / sizeof(T); }
+
+// The 16 bytes of vector v as f32; elements from `cols` on are zero.
+template <typename T>
+__device__ __forceinline__ void vec_to_f32(const uint4& raw, float* f) {
+    if constexpr (sizeof(T) == 4) {
+        f[0] = __uint_as_float(raw.x); f[1] = __uint_as_float(raw.y);
+        f[2] = __uint_as_float(raw.z); f[3] = __uint_as_float(raw.w);
+    } else {
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (std::is_same<T, __half>::value) {
+                const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                f[2 * i] = p.x; f[2 * i + 1] = p.y;
+            } else {                                 // bf16 is the upper half of f32
+                f[2 * i] = __uint_as_float(w[i] << 16);
+                f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+            }
+        }
+    }
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ uint4 f32_to_vec(const float* f) {
+    if constexpr (sizeof(T) == 4)
+        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    else
+        return make_uint4(pack2(f[0], f[1], T()), pack2(f[2], f[3], T()), pack2(f[4], f[5], T()), pack2(f[6], f[7], T()));
+}
+// Elements [at, at + vec_elems) of a row; past the row's end zeros, read one by one.
+template <typename T>
+__device__ __forceinline__ uint4 load_vec(const T* row, uint32_t at, uint32_t cols) {
+    constexpr uint32_t E = vec_elems<T>();
+    if (at + E <= cols) return *reinterpret_cast<const uint4*>(row + at);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (at < cols) {
+        T e[E];
+        *reinterpret_cast<uint4*>(e) = v;
+        for (uint32_t i = 0; i < E; i++)
+            if (at + i < cols) e[i] = row[at + i];
+        v = *reinterpret_cast<uint4*>(e);
+    }
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ void store_vec(T* row, uint32_t at, uint32_t cols, const uint4& v) {
+    constexpr uint32_t E = vec_elems<T>();
+    if (at + E <= cols) {
+        *reinterpret_cast<uint4*>(row + at) = v;
+        return;
+    }
+    const T* e = reinterpret_cast<const T*>(&v);
+    for (uint32_t i = 0; i < E; i++)
+        if (at + i < cols) row[at + i] = e[i];
+}
+
+// Adding 1.5 * 2^23 leaves an f32 of magnitude below 2^22, rounded to the nearest
+// integer (ties to even), in the low mantissa bits: the low byte is the int8.
+constexpr float kRound = 12582912.0f;
+__device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d) {
+    const uint32_t ab = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040);
+    const uint32_t cd = __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040);
+    return __byte_perm(ab, cd, 0x5410);
+}
+
+// E values of a row, times f (127 / max, or what maps onto it), to int8 at q + at.
+// `r` decides for rows whose scale is zero, not finite or subnormal; y maps a
+// value to what r.scale stands for.
+template <uint32_t E, typename Y>
+__device__ __forceinline__ void store_quant(int8_t* q, uint32_t at, uint32_t cols, const float* v, float f,
+                                            const RowScale& r, Y y) {
+    uint32_t w[E / 4];
+    if (!r.tiny && !r.zero) {
+#pragma unroll
+        for (uint32_t i = 0; i < E / 4; i++)
+            w[i] = low_bytes(fmaf(v[4 * i], f, kRound), fmaf(v[4 * i + 1], f, kRound), fmaf(v[4 * i + 2], f, kRound),
+                             fmaf(v[4 * i + 3], f, kRound));
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < E / 4; i++) {
+            w[i] = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) w[i] |= ((uint32_t)quant1(y(v[4 * i + j]), r) & 0xFFu) << (8 * j);
+        }
+    }
+    if (at + E <= cols) {
+        if constexpr (E == 8) *reinterpret_cast<uint2*>(q + at) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t*>(q + at) = w[0];
+    } else {
+        for (uint32_t i = 0; i < E; i++)
+            if (at + i < cols) q[at + i] = (int8_t)(w[i >> 2] >> (8 * (i & 3u)));
+    }
+}
+
+// Maximum and sum over the G threads of a row; every thread gets both, and each
+// thread adds in the same order. `turn` alternates between two halves of red, so
+// that one barrier a row is enough.
+template <uint32_t G>
+__device__ __forceinline__ void row_max_sum(uint32_t& m, float& s, uint32_t* red, uint32_t turn) {
+    m = __reduce_max_sync(0xffffffffu, m);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if constexpr (G > 32) {
+        constexpr uint32_t W = G / 32;
+        uint32_t* r = red + (turn & 1u) * 2 * W;
+        if ((threadIdx.x & 31u) == 0) {
+            r[threadIdx.x >> 5] = m;
+            r[W + (threadIdx.x >> 5)] = __float_as_uint(s);
+        }
+        __syncthreads();
+        m = r[0];
+        s = __uint_as_float(r[W]);
+#pragma unroll
+        for (uint32_t i = 1; i < W; i++) {
+            m = max(m, r[i]);
+            s += __uint_as_float(r[W + i]);
+        }
     }
 }
 

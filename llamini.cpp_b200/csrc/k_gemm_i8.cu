@@ -470,15 +470,6 @@ __device__ __forceinline__ void tmem_get32(uint32_t taddr, int* r) {
                    "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // The tile a pair works on at step t: groups of up to 8 token tiles, within
 // a group the token tile changes fastest, so that the tiles in flight share
 // rows of both operands in L2. From step `whole` on, two steps to a tile.

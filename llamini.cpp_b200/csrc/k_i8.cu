@@ -6,9 +6,14 @@
 // norm the sum of squares), then the rounding to int8 (i8.cuh). Sums, scales
 // and every value before the rounding are f32.
 #include "i8.cuh"
+#include "pdl.cuh"
+
+#include <atomic>
 
 namespace lm {
 namespace {
+
+constexpr uint32_t kWarpRows = 8;          // rows at a time of a CTA whose warps have one each
 
 // ---------------------------------------------------------------- norm
 
@@ -53,6 +58,73 @@ __global__ void __launch_bounds__(256) norm_i8_kernel(const NormArgs a) {
     if (threadIdx.x == 0) a.scale[row] = s.scale;
 }
 
+// The same with a row in the registers of G threads (V vectors each), read once:
+// h w of every element is kept from the first pass to the second. CTAs walk the
+// rows with w in registers and the next row's loads in flight.
+template <typename T, uint32_t G, uint32_t V, bool RESID>
+__global__ void __launch_bounds__(G == 32 ? 32 * kWarpRows : G) norm_i8_rows_kernel(const NormArgs a) {
+    constexpr uint32_t E = vec_elems<T>();
+    constexpr uint32_t R = G == 32 ? kWarpRows : 1;  // rows of a CTA at a time
+    __shared__ uint32_t red[G == 32 ? 1 : 4 * (G / 32)];
+    const uint32_t t = G == 32 ? threadIdx.x & 31u : threadIdx.x;
+    uint64_t row = (uint64_t)blockIdx.x * R + (G == 32 ? threadIdx.x >> 5 : 0);
+    const uint64_t step = (uint64_t)gridDim.x * R;
+    pdl_trigger();
+    pdl_wait();
+    float w[V][E];
+#pragma unroll
+    for (uint32_t j = 0; j < V; j++)
+#pragma unroll
+        for (uint32_t i = 0; i < E; i += 4) {
+            const uint4 v = load_vec<float>(a.w, (t + j * G) * E + i, a.cols);
+            vec_to_f32<float>(v, &w[j][i]);
+        }
+    uint4 x[V], r[V];
+    auto load = [&](uint64_t at) {
+        const T* px = static_cast<const T*>(a.x) + at * a.ld_x;
+        const T* pr = static_cast<const T*>(a.resid) + at * a.ld_resid;
+#pragma unroll
+        for (uint32_t j = 0; j < V; j++) {
+            x[j] = load_vec<T>(px, (t + j * G) * E, a.cols);
+            if (RESID) r[j] = load_vec<T>(pr, (t + j * G) * E, a.cols);
+        }
+    };
+    if (row < a.rows) load(row);
+    for (uint32_t turn = 0; row < a.rows; row += step, turn++) {
+        float hw[V][E];
+        uint32_t m = 0;
+        float ss = 0.f;
+        T* o = a.sum ? static_cast<T*>(a.sum) + row * a.ld_sum : nullptr;
+#pragma unroll
+        for (uint32_t j = 0; j < V; j++) {
+            vec_to_f32<T>(x[j], hw[j]);
+            if (RESID) {
+                float f[E];
+                vec_to_f32<T>(r[j], f);
+#pragma unroll
+                for (uint32_t i = 0; i < E; i++) hw[j][i] += f[i];
+            }
+            if (o) store_vec<T>(o, (t + j * G) * E, a.cols, f32_to_vec<T>(hw[j]));
+#pragma unroll
+            for (uint32_t i = 0; i < E; i++) {
+                ss = fmaf(hw[j][i], hw[j][i], ss);
+                hw[j][i] *= w[j][i];
+                m = max(m, abs_bits(hw[j][i]));
+            }
+        }
+        if (row + step < a.rows) load(row + step);
+        row_max_sum<G>(m, ss, red, turn);
+        const float rstd = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
+        RowScale s = row_scale(__uint_as_float(m) * rstd);
+        const float f = rstd * s.inv;
+        s.tiny |= !(f < INFINITY);
+#pragma unroll
+        for (uint32_t j = 0; j < V; j++)
+            store_quant<E>(a.q + row * a.ld_q, (t + j * G) * E, a.cols, hw[j], f, s, [&](float v) { return v * rstd; });
+        if (t == 0) a.scale[row] = s.scale;
+    }
+}
+
 // ---------------------------------------------------------------- gated activation
 
 struct GluArgs {
@@ -64,13 +136,16 @@ struct GluArgs {
     uint32_t rows, cols, act;
 };
 
-// The activations of model.c:14-25 (and gpt2.c's gelu), in f32.
+// The activations of model.c:14-25 (and gpt2.c's gelu), in f32. GELU's (1 +
+// tanh z) / 2 is 1 / (1 + exp(-2 z)), which does not cancel for negative z and
+// costs one exponential. The quotients use the approximate division (2 ulp): the
+// result is rounded to 8 bits.
 template <uint32_t ACT>
 __device__ __forceinline__ float activate(float x) {
-    if (ACT == ACT_SILU) return x / (1.0f + expf(-x));
+    if (ACT == ACT_SILU) return __fdividef(x, 1.0f + expf(-x));
     if (ACT == ACT_GELU) {
-        const float k0 = 0.79788456080286535587989211986876f;
-        return 0.5f * x * (1.0f + tanhf(k0 * x * (1.0f + 0.044715f * x * x)));
+        const float k0 = 2.0f * 0.79788456080286535587989211986876f;
+        return __fdividef(x, 1.0f + expf(-k0 * x * (1.0f + 0.044715f * x * x)));
     }
     return x;
 }
@@ -90,6 +165,55 @@ __global__ void __launch_bounds__(256) glu_i8_kernel(const GluArgs a) {
     for (uint32_t i = threadIdx.x; i < a.cols; i += blockDim.x)
         a.q[row * a.ld_q + i] = (int8_t)quant1(activate<ACT>(to_f32(g[i])) * (u ? to_f32(u[i]) : 1.f), s);
     if (threadIdx.x == 0) a.scale[row] = s.scale;
+}
+
+// The same with a row's values in the registers of G threads, read and
+// activated once; the next row's loads are in flight meanwhile.
+template <typename T, uint32_t ACT, bool UP, uint32_t G, uint32_t V>
+__global__ void __launch_bounds__(G == 32 ? 32 * kWarpRows : G) glu_i8_rows_kernel(const GluArgs a) {
+    constexpr uint32_t E = vec_elems<T>();
+    constexpr uint32_t R = G == 32 ? kWarpRows : 1;
+    __shared__ uint32_t red[G == 32 ? 1 : 4 * (G / 32)];
+    const uint32_t t = G == 32 ? threadIdx.x & 31u : threadIdx.x;
+    uint64_t row = (uint64_t)blockIdx.x * R + (G == 32 ? threadIdx.x >> 5 : 0);
+    const uint64_t step = (uint64_t)gridDim.x * R;
+    pdl_trigger();
+    pdl_wait();
+    uint4 g[V], u[V];
+    auto load = [&](uint64_t at) {
+        const T* pg = static_cast<const T*>(a.gate) + at * a.ld_gate;
+        const T* pu = static_cast<const T*>(a.up) + at * a.ld_up;
+#pragma unroll
+        for (uint32_t j = 0; j < V; j++) {
+            g[j] = load_vec<T>(pg, (t + j * G) * E, a.cols);
+            if (UP) u[j] = load_vec<T>(pu, (t + j * G) * E, a.cols);
+        }
+    };
+    if (row < a.rows) load(row);
+    for (uint32_t turn = 0; row < a.rows; row += step, turn++) {
+        float y[V][E];
+        uint32_t m = 0;
+        float unused = 0.f;
+#pragma unroll
+        for (uint32_t j = 0; j < V; j++) {
+            vec_to_f32<T>(g[j], y[j]);
+            float f[E];
+            if (UP) vec_to_f32<T>(u[j], f);
+#pragma unroll
+            for (uint32_t i = 0; i < E; i++) {
+                y[j][i] = activate<ACT>(y[j][i]);
+                if (UP) y[j][i] *= f[i];
+                m = max(m, abs_bits(y[j][i]));
+            }
+        }
+        if (row + step < a.rows) load(row + step);
+        row_max_sum<G>(m, unused, red, turn);
+        const RowScale s = row_scale(__uint_as_float(m));
+#pragma unroll
+        for (uint32_t j = 0; j < V; j++)
+            store_quant<E>(a.q + row * a.ld_q, (t + j * G) * E, a.cols, y[j], s.inv, s, [](float v) { return v; });
+        if (t == 0) a.scale[row] = s.scale;
+    }
 }
 
 // ---------------------------------------------------------------- weights
@@ -339,15 +463,92 @@ bool align_ok(const char* who, const void* const* ptrs, int n, size_t bytes) {
     return true;
 }
 
-template <typename T>
-bool launch_glu(const GluArgs& a, cudaStream_t st) {
-    if (a.act == ACT_SILU) glu_i8_kernel<T, ACT_SILU><<<a.rows, 256, 0, st>>>(a);
-    else if (a.act == ACT_GELU) glu_i8_kernel<T, ACT_GELU><<<a.rows, 256, 0, st>>>(a);
-    else glu_i8_kernel<T, LLAMINI_ACT_NONE><<<a.rows, 256, 0, st>>>(a);
+// CTAs of a kernel that walks `rows` rows, `per` at a time: as many as run at
+// once, and no more than there are rows.
+template <typename K>
+uint32_t walkers(std::atomic<uint32_t>& memo, K* kernel, uint32_t threads, uint64_t rows, uint32_t per) {
+    uint32_t n = memo.load(std::memory_order_relaxed);
+    if (n == 0) {
+        int dev = 0, sms = 0, occ = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kernel, (int)threads, 0) != cudaSuccess || sms * occ <= 0) {
+            cudaGetLastError();
+            sms = 148;
+            occ = 1;
+        }
+        n = (uint32_t)(sms * occ);
+        memo.store(n, std::memory_order_relaxed);
+    }
+    const uint64_t want = (rows + per - 1) / per;
+    return (uint32_t)(want < n ? want : n);
+}
+template <typename T> bool vec_rows(const void* p, uint64_t ld) {
+    return !p || (i8_aligned(p, 16) && ld * sizeof(T) % 16 == 0);
+}
+template <typename T> bool vec_q(const int8_t* q, uint64_t ld) {
+    return i8_aligned(q, vec_elems<T>()) && ld % vec_elems<T>() == 0;
+}
+
+template <typename T, uint32_t G, uint32_t V, bool RESID>
+bool launch_norm_rows(const NormArgs& a, cudaStream_t st) {
+    static std::atomic<uint32_t> memo{0};
+    constexpr uint32_t threads = G == 32 ? 32 * kWarpRows : G, per = G == 32 ? kWarpRows : 1;
+    const uint32_t grid = walkers(memo, norm_i8_rows_kernel<T, G, V, RESID>, threads, a.rows, per);
+    return LM_CUDA(launch_k(norm_i8_rows_kernel<T, G, V, RESID>, dim3(grid), dim3(threads), 0, st, a));
+}
+template <typename T, uint32_t G, uint32_t V>
+bool launch_norm_rows(const NormArgs& a, cudaStream_t st) {
+    return a.resid ? launch_norm_rows<T, G, V, true>(a, st) : launch_norm_rows<T, G, V, false>(a, st);
+}
+template <typename T, uint32_t ACT, uint32_t G, uint32_t V>
+bool launch_glu_rows(const GluArgs& a, cudaStream_t st) {
+    static std::atomic<uint32_t> memo{0}, memo1{0};
+    constexpr uint32_t threads = G == 32 ? 32 * kWarpRows : G, per = G == 32 ? kWarpRows : 1;
+    if (a.up) {
+        const uint32_t grid = walkers(memo, glu_i8_rows_kernel<T, ACT, true, G, V>, threads, a.rows, per);
+        return LM_CUDA(launch_k(glu_i8_rows_kernel<T, ACT, true, G, V>, dim3(grid), dim3(threads), 0, st, a));
+    }
+    const uint32_t grid = walkers(memo1, glu_i8_rows_kernel<T, ACT, false, G, V>, threads, a.rows, per);
+    return LM_CUDA(launch_k(glu_i8_rows_kernel<T, ACT, false, G, V>, dim3(grid), dim3(threads), 0, st, a));
+}
+
+// Threads a row and vectors a thread. Many short rows: a warp each; otherwise the
+// smallest CTA that holds the row in up to 4 vectors a thread. Rows past 4096
+// vectors, and pitches or bases that are not whole vectors, take the two-pass
+// kernel.
+#define LM_I8_ROWS(LAUNCH, ...)                                              \
+    do {                                                                     \
+        const uint32_t nv = (a.cols + vec_elems<T>() - 1) / vec_elems<T>();  \
+        if (a.rows >= 1024 && nv <= 32) return LAUNCH<__VA_ARGS__, 32, 1>(a, st);  \
+        if (a.rows >= 1024 && nv <= 64) return LAUNCH<__VA_ARGS__, 32, 2>(a, st);  \
+        if (a.rows >= 1024 && nv <= 128) return LAUNCH<__VA_ARGS__, 32, 4>(a, st); \
+        if (nv <= 128) return LAUNCH<__VA_ARGS__, 128, 1>(a, st);            \
+        if (nv <= 256) return LAUNCH<__VA_ARGS__, 128, 2>(a, st);            \
+        if (nv <= 512) return LAUNCH<__VA_ARGS__, 256, 2>(a, st);            \
+        if (nv <= 1024) return LAUNCH<__VA_ARGS__, 512, 2>(a, st);           \
+        if (nv <= 1536) return LAUNCH<__VA_ARGS__, 512, 3>(a, st);           \
+        if (nv <= 2048) return LAUNCH<__VA_ARGS__, 512, 4>(a, st);           \
+        if (nv <= 4096) return LAUNCH<__VA_ARGS__, 1024, 4>(a, st);          \
+    } while (0)
+
+template <typename T, uint32_t ACT>
+bool launch_glu_act(const GluArgs& a, cudaStream_t st) {
+    if (vec_rows<T>(a.gate, a.ld_gate) && vec_rows<T>(a.up, a.ld_up) && vec_q<T>(a.q, a.ld_q))
+        LM_I8_ROWS(launch_glu_rows, T, ACT);
+    glu_i8_kernel<T, ACT><<<a.rows, 256, 0, st>>>(a);
     return LM_CUDA(cudaGetLastError());
 }
 template <typename T>
+bool launch_glu(const GluArgs& a, cudaStream_t st) {
+    if (a.act == ACT_SILU) return launch_glu_act<T, ACT_SILU>(a, st);
+    if (a.act == ACT_GELU) return launch_glu_act<T, ACT_GELU>(a, st);
+    return launch_glu_act<T, LLAMINI_ACT_NONE>(a, st);
+}
+template <typename T>
 bool launch_norm(const NormArgs& a, cudaStream_t st) {
+    if (vec_rows<T>(a.x, a.ld_x) && vec_rows<T>(a.resid, a.ld_resid) && vec_rows<T>(a.sum, a.ld_sum) &&
+        i8_aligned(a.w, 16) && vec_q<T>(a.q, a.ld_q))
+        LM_I8_ROWS(launch_norm_rows, T);
     norm_i8_kernel<T><<<a.rows, 256, 0, st>>>(a);
     return LM_CUDA(cudaGetLastError());
 }
