@@ -102,9 +102,10 @@ int llamini_causal_mha_noalloc(const f32* d_q, const f32* d_key, const f32* d_va
  * A decoder layer's matrices as int8 x int8 products on the tensor cores: int8
  * weights with one scale for each output channel, activations with one scale
  * for each token. A row q[0..cols) with its scale stands for the values
- * q[i] * scale, where scale = max|y| / 127 and q = y / scale rounded to the
- * nearest integer, ties to even. A row of zeros has scale 0; a row that holds a
- * NaN or an infinity has scale NaN and q = 0.
+ * q[i] * scale, where scale = max|y| / 127 and q = y * (127 / max|y|) rounded to
+ * the nearest integer, ties to even (both quotients rounded to f32; y / scale,
+ * kept within -127 to 127, where max|y| is below 1.5e-36). A row of zeros has scale
+ * 0; a row that holds a NaN or an infinity has scale NaN and q = 0.
  *
  * Every call takes DEVICE buffers of the calling thread's current device (others
  * are refused) and enqueues its work on `stream` (a cudaStream_t; NULL = the
@@ -124,9 +125,8 @@ int llamini_causal_mha_noalloc(const f32* d_q, const f32* d_key, const f32* d_va
 #define LLAMINI_ACT_NONE 2
 
 /* int8 rows of raw GGUF blocks: the `cols` elements of each of `rows` rows,
- * decoded as by llamini_dequant_device (bit-identical to gguf.c:409-594), get
- * the row's scale; q is the exact nearest integer of w / scale. d_blocks holds
- * whole rows back to back (2-byte aligned; F32 4-byte), d_q is rows x ld_q, d_scale
+ * decoded as by llamini_dequant_device (bit-identical to gguf.c:409-594), and the
+ * row's scale. d_blocks holds whole rows back to back (2-byte aligned; F32 4-byte), d_q is rows x ld_q, d_scale
  * holds `rows` floats. Done once per matrix, when a model is loaded. */
 int llamini_weights_i8_device(u32 type, const void* d_blocks, u32 rows, u32 cols,
                               i8* d_q, u64 ld_q, f32* d_scale, void* stream);

@@ -3,10 +3,14 @@
 // a row of f32 values to int8.
 //
 // An int8 row stands for the values q[i] * scale with one f32 scale a row:
-// scale = max|y| / 127 and q = y / scale rounded to the nearest integer, ties
-// to even, so |q| <= 127 and -128 never appears. A row of zeros has scale 0. A
-// row that holds a NaN or an infinity has scale NaN and q = 0: every value it
-// stands for is NaN, so the fault stays visible.
+// scale = max|y| / 127 and q = y * (127 / max|y|) rounded to the nearest integer,
+// ties to even, both quotients rounded to f32, so |q| <= 127 and -128 never
+// appears. (The reciprocal instead of y / scale moves only an element that lies
+// within 2^-16 of halfway between two integers, and makes the rounding of y one
+// fused multiply-add, exact and the same everywhere.) A row of zeros has scale 0.
+// A row that holds a NaN or an infinity has scale NaN and q = 0: every value it
+// stands for is NaN, so the fault stays visible. Where 127 / max|y| would
+// overflow (max|y| below 1.5e-36) q is y / scale instead, within -127 to 127.
 #pragma once
 
 #include "internal.h"
@@ -54,6 +58,20 @@ inline bool i8_device_ptrs(const char* who, const void* const* ptrs, int n) {
     return true;
 }
 
+// SMs of the device (of the first one a call is made on: all of a box are alike).
+inline uint32_t i8_sms() {
+    static const uint32_t sms = [] {
+        int dev = 0, n = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess ||
+            cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 2) {
+            cudaGetLastError();
+            n = 148;
+        }
+        return (uint32_t)n;
+    }();
+    return sms;
+}
+
 inline bool i8_aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 // ---------------------------------------------------------------- device
@@ -70,6 +88,16 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
 // magnitudes, infinity above every finite value and every NaN above that, so
 // an integer maximum over a row also finds its NaNs.
 __device__ __forceinline__ uint32_t abs_bits(float y) { return __float_as_uint(y) & 0x7FFFFFFFu; }
+// max(m, |y|), NaN when either is: one instruction an element.
+__device__ __forceinline__ float max_abs(float m, float y) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(m), "f"(fabsf(y)));
+    return r;
+}
+
+// Adding 1.5 * 2^23 leaves an f32 of magnitude below 2^22, rounded to the nearest
+// integer (ties to even), in the low mantissa bits: the low byte is the int8.
+constexpr float kRound = 12582912.0f;
 
 // The scale of a row whose largest magnitude has these bits, and how its
 // elements become integers.
@@ -87,12 +115,11 @@ __device__ __forceinline__ RowScale row_scale(float amax) {
     r.inv = r.tiny || bad ? 0.0f : __fdiv_rn(127.0f, amax);
     return r;
 }
-// One element: y * (127 / max) instead of y / scale, one rounding apart, which
-// only moves an element that lies within 2^-17 of halfway between two integers.
+// One element of a row.
 __device__ __forceinline__ int quant1(float y, const RowScale& r) {
     if (r.zero) return 0;
     if (r.tiny) return max(-127, min(127, __float2int_rn(__fdiv_rn(y, r.scale))));
-    return __float2int_rn(y * r.inv);
+    return (int)(int8_t)__float_as_uint(fmaf(y, r.inv, kRound));
 }
 
 // Block-wide maximum of unsigned integers and sum of floats; every thread gets
@@ -118,8 +145,8 @@ __device__ __forceinline__ void block_max_sum(uint32_t& m, float& s, uint32_t* r
 
 // ---------------------------------------------------------------- rows in registers
 //
-// A row of 16-byte vectors spread over G threads (a warp, or a whole CTA), V
-// vectors a thread, vector j of thread t at t + j G.
+// A row of 16-byte vectors spread over G threads (a warp, or a whole CTA), up to
+// V vectors a thread, vector j of thread t at t + j G.
 
 template <typename T> constexpr uint32_t vec_elems() { return 16 / sizeof(T); }
 
@@ -185,9 +212,6 @@ __device__ __forceinline__ void store_vec(T* row, uint32_t at, uint32_t cols, co
         if (at + i < cols) row[at + i] = e[i];
 }
 
-// Adding 1.5 * 2^23 leaves an f32 of magnitude below 2^22, rounded to the nearest
-// integer (ties to even), in the low mantissa bits: the low byte is the int8.
-constexpr float kRound = 12582912.0f;
 __device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d) {
     const uint32_t ab = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040);
     const uint32_t cd = __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040);
@@ -223,29 +247,27 @@ __device__ __forceinline__ void store_quant(int8_t* q, uint32_t at, uint32_t col
     }
 }
 
-// Maximum and sum over the G threads of a row; every thread gets both, and each
-// thread adds in the same order. `turn` alternates between two halves of red, so
-// that one barrier a row is enough.
-template <uint32_t G>
+// Maximum and sum over the threads of a row, a warp (WARP) or the CTA; every
+// thread gets both, and each adds in the same order. `turn` alternates between
+// two halves of red (128 words), so that one barrier a row is enough.
+template <bool WARP>
 __device__ __forceinline__ void row_max_sum(uint32_t& m, float& s, uint32_t* red, uint32_t turn) {
     m = __reduce_max_sync(0xffffffffu, m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if constexpr (G > 32) {
-        constexpr uint32_t W = G / 32;
-        uint32_t* r = red + (turn & 1u) * 2 * W;
-        if ((threadIdx.x & 31u) == 0) {
+    if constexpr (!WARP) {
+        const uint32_t nw = blockDim.x >> 5, lane = threadIdx.x & 31u;
+        uint32_t* r = red + (turn & 1u) * 64;
+        if (lane == 0) {
             r[threadIdx.x >> 5] = m;
-            r[W + (threadIdx.x >> 5)] = __float_as_uint(s);
+            r[32 + (threadIdx.x >> 5)] = __float_as_uint(s);
         }
         __syncthreads();
-        m = r[0];
-        s = __uint_as_float(r[W]);
+        m = lane < nw ? r[lane] : 0u;
+        s = lane < nw ? __uint_as_float(r[32 + lane]) : 0.f;
+        m = __reduce_max_sync(0xffffffffu, m);
 #pragma unroll
-        for (uint32_t i = 1; i < W; i++) {
-            m = max(m, r[i]);
-            s += __uint_as_float(r[W + i]);
-        }
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     }
 }
 

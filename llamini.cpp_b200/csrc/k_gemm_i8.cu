@@ -735,17 +735,6 @@ bool operand_map(CUtensorMap* m, const int8_t* p, uint64_t ld, uint32_t rows, ui
     return false;
 }
 
-uint32_t device_sms() {
-    static const uint32_t sms = [] {
-        int dev = 0, n = 0;
-        if (cudaGetDevice(&dev) != cudaSuccess ||
-            cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-            n = 148;
-        return (uint32_t)n;
-    }();
-    return sms;
-}
-
 // Launch with thread-block clusters of `cluster` CTAs (0: the kernel's own
 // size) and programmatic
 // dependent launch (the kernels wait before their first read of the inputs).
@@ -797,7 +786,7 @@ bool launch_few(const GemmI8Args& g, cudaStream_t st) {
     // stages: 6.2 us in one part, 4.7 in four or eight; 172 tiles of 32: 21.1 us in
     // one part, 31.9 in two, which no longer run at once)
     uint32_t cs = 1;
-    while (cs < 8 && tiles * cs * 2 <= 2 * device_sms() && nkb / (cs * 2) >= 2) cs *= 2;
+    while (cs < 8 && tiles * cs * 2 <= 2 * i8_sms() && nkb / (cs * 2) >= 2) cs *= 2;
     if (tiles * cs > 0x7FFFFFFFull) {
         set_error("gemm_i8: %u x %u outputs are too many for one call", g.m, g.n);
         return false;
@@ -829,7 +818,7 @@ template <typename T, bool TMA_OUT>
 bool launch_many(const GemmI8Args& g, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};
     if (!allow_smem(ready, gemm_i8_many_kernel<T, TMA_OUT>, Many::kSmem)) return false;
-    const uint64_t tm = (g.m + 255) / 256, tn = (g.n + 255) / 256, n = tm * tn, pairs = device_sms() / 2;
+    const uint64_t tm = (g.m + 255) / 256, tn = (g.n + 255) / 256, n = tm * tn, pairs = i8_sms() / 2;
     if (n > 0x3FFFFFFFull) {
         set_error("gemm_i8: %u x %u outputs are too many for one call", g.m, g.n);
         return false;
@@ -867,7 +856,7 @@ bool tma_rows(const GemmI8Args& g) {
 template <typename T>
 bool launch(const GemmI8Args& g, cudaStream_t st) {
     if (!tma_rows(g)) return launch_any<T>(g, st);
-    const uint64_t tn = (g.n + 127) / 128, sms = device_sms();
+    const uint64_t tn = (g.n + 127) / 128, sms = i8_sms();
     const uint32_t nkb = (g.k + kSlab - 1) / kSlab;
     const uint64_t wide = 6 * sms / 5, most = nkb < 30 ? wide : 3 * sms / 5;
     uint32_t nt = 16;

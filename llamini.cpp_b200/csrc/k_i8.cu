@@ -9,11 +9,14 @@
 #include "pdl.cuh"
 
 #include <atomic>
+#include <cstdlib>
 
 namespace lm {
 namespace {
 
 constexpr uint32_t kWarpRows = 8;          // rows at a time of a CTA whose warps have one each
+// The most threads of a CTA that keeps up to V vectors a thread in registers.
+template <bool WARP, uint32_t V> constexpr uint32_t rows_threads() { return WARP ? 32 * kWarpRows : V > 1 ? 512 : 1024; }
 
 // ---------------------------------------------------------------- norm
 
@@ -61,13 +64,14 @@ __global__ void __launch_bounds__(256) norm_i8_kernel(const NormArgs a) {
 // The same with a row in the registers of G threads (V vectors each), read once:
 // h w of every element is kept from the first pass to the second. CTAs walk the
 // rows with w in registers and the next row's loads in flight.
-template <typename T, uint32_t G, uint32_t V, bool RESID>
-__global__ void __launch_bounds__(G == 32 ? 32 * kWarpRows : G) norm_i8_rows_kernel(const NormArgs a) {
+template <typename T, bool RESID, bool WARP, uint32_t V>
+__global__ void __launch_bounds__(rows_threads<WARP, V>()) norm_i8_rows_kernel(const NormArgs a) {
     constexpr uint32_t E = vec_elems<T>();
-    constexpr uint32_t R = G == 32 ? kWarpRows : 1;  // rows of a CTA at a time
-    __shared__ uint32_t red[G == 32 ? 1 : 4 * (G / 32)];
-    const uint32_t t = G == 32 ? threadIdx.x & 31u : threadIdx.x;
-    uint64_t row = (uint64_t)blockIdx.x * R + (G == 32 ? threadIdx.x >> 5 : 0);
+    constexpr uint32_t R = WARP ? kWarpRows : 1;     // rows of a CTA at a time
+    constexpr bool AHEAD = V * E <= 32;              // the next row's vectors fit the registers too
+    __shared__ uint32_t red[WARP ? 1 : 128];
+    const uint32_t G = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31u : threadIdx.x;
+    uint64_t row = (uint64_t)blockIdx.x * R + (WARP ? threadIdx.x >> 5 : 0);
     const uint64_t step = (uint64_t)gridDim.x * R;
     pdl_trigger();
     pdl_wait();
@@ -89,11 +93,11 @@ __global__ void __launch_bounds__(G == 32 ? 32 * kWarpRows : G) norm_i8_rows_ker
             if (RESID) r[j] = load_vec<T>(pr, (t + j * G) * E, a.cols);
         }
     };
-    if (row < a.rows) load(row);
+    if (AHEAD && row < a.rows) load(row);
     for (uint32_t turn = 0; row < a.rows; row += step, turn++) {
+        if (!AHEAD) load(row);
         float hw[V][E];
-        uint32_t m = 0;
-        float ss = 0.f;
+        float top = 0.f, ss = 0.f;
         T* o = a.sum ? static_cast<T*>(a.sum) + row * a.ld_sum : nullptr;
 #pragma unroll
         for (uint32_t j = 0; j < V; j++) {
@@ -109,11 +113,12 @@ __global__ void __launch_bounds__(G == 32 ? 32 * kWarpRows : G) norm_i8_rows_ker
             for (uint32_t i = 0; i < E; i++) {
                 ss = fmaf(hw[j][i], hw[j][i], ss);
                 hw[j][i] *= w[j][i];
-                m = max(m, abs_bits(hw[j][i]));
+                top = max_abs(top, hw[j][i]);
             }
         }
-        if (row + step < a.rows) load(row + step);
-        row_max_sum<G>(m, ss, red, turn);
+        if (AHEAD && row + step < a.rows) load(row + step);
+        uint32_t m = abs_bits(top);
+        row_max_sum<WARP>(m, ss, red, turn);
         const float rstd = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
         RowScale s = row_scale(__uint_as_float(m) * rstd);
         const float f = rstd * s.inv;
@@ -169,13 +174,14 @@ __global__ void __launch_bounds__(256) glu_i8_kernel(const GluArgs a) {
 
 // The same with a row's values in the registers of G threads, read and
 // activated once; the next row's loads are in flight meanwhile.
-template <typename T, uint32_t ACT, bool UP, uint32_t G, uint32_t V>
-__global__ void __launch_bounds__(G == 32 ? 32 * kWarpRows : G) glu_i8_rows_kernel(const GluArgs a) {
+template <typename T, uint32_t ACT, bool UP, bool WARP, uint32_t V>
+__global__ void __launch_bounds__(rows_threads<WARP, V>()) glu_i8_rows_kernel(const GluArgs a) {
     constexpr uint32_t E = vec_elems<T>();
-    constexpr uint32_t R = G == 32 ? kWarpRows : 1;
-    __shared__ uint32_t red[G == 32 ? 1 : 4 * (G / 32)];
-    const uint32_t t = G == 32 ? threadIdx.x & 31u : threadIdx.x;
-    uint64_t row = (uint64_t)blockIdx.x * R + (G == 32 ? threadIdx.x >> 5 : 0);
+    constexpr uint32_t R = WARP ? kWarpRows : 1;
+    constexpr bool AHEAD = V * E <= 32;
+    __shared__ uint32_t red[WARP ? 1 : 128];
+    const uint32_t G = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31u : threadIdx.x;
+    uint64_t row = (uint64_t)blockIdx.x * R + (WARP ? threadIdx.x >> 5 : 0);
     const uint64_t step = (uint64_t)gridDim.x * R;
     pdl_trigger();
     pdl_wait();
@@ -189,11 +195,11 @@ __global__ void __launch_bounds__(G == 32 ? 32 * kWarpRows : G) glu_i8_rows_kern
             if (UP) u[j] = load_vec<T>(pu, (t + j * G) * E, a.cols);
         }
     };
-    if (row < a.rows) load(row);
+    if (AHEAD && row < a.rows) load(row);
     for (uint32_t turn = 0; row < a.rows; row += step, turn++) {
+        if (!AHEAD) load(row);
         float y[V][E];
-        uint32_t m = 0;
-        float unused = 0.f;
+        float top = 0.f, unused = 0.f;
 #pragma unroll
         for (uint32_t j = 0; j < V; j++) {
             vec_to_f32<T>(g[j], y[j]);
@@ -203,11 +209,12 @@ __global__ void __launch_bounds__(G == 32 ? 32 * kWarpRows : G) glu_i8_rows_kern
             for (uint32_t i = 0; i < E; i++) {
                 y[j][i] = activate<ACT>(y[j][i]);
                 if (UP) y[j][i] *= f[i];
-                m = max(m, abs_bits(y[j][i]));
+                top = max_abs(top, y[j][i]);
             }
         }
-        if (row + step < a.rows) load(row + step);
-        row_max_sum<G>(m, unused, red, turn);
+        if (AHEAD && row + step < a.rows) load(row + step);
+        uint32_t m = abs_bits(top);
+        row_max_sum<WARP>(m, unused, red, turn);
         const RowScale s = row_scale(__uint_as_float(m));
 #pragma unroll
         for (uint32_t j = 0; j < V; j++)
@@ -228,6 +235,7 @@ struct WeightArgs {
 };
 
 constexpr uint32_t kWSeg = 48 * 1024;      // raw bytes of a row staged at a time
+constexpr uint32_t kWRow = 96 * 1024;      // longest row that is staged whole
 constexpr uint32_t kWSlack = 192;          // behind it: the offset modulo 16, and a short last unit decoded whole
 constexpr uint32_t kWThreads = 256;
 
@@ -351,20 +359,6 @@ __host__ __device__ constexpr uint32_t block_bytes(uint32_t t) {
          : t == GGML_TYPE_Q5_K ? 176 : 210;
 }
 
-// w / s rounded to the nearest integer, ties to even, exactly: the estimate
-// w * (127 / max) is within one of it, and the remainder w - q s comes from one
-// fused multiply-add, exact near s / 2 (there it is a multiple of half an ulp
-// of s and below s). Load-time work, so the int8 weights of a file are the
-// same everywhere.
-__device__ __forceinline__ int quant_exact(float w, const RowScale& r) {
-    if (r.zero || r.tiny) return quant1(w, r);
-    int q = __float2int_rn(w * r.inv);
-    const float rem = fmaf(-(float)q, r.scale, w), half = 0.5f * r.scale;
-    if (rem > half || (rem == half && (q & 1))) q++;
-    else if (rem < -half || (rem == -half && (q & 1))) q--;
-    return q;
-}
-
 // Segment `s0` (units) of a row into shared memory, at the same offset modulo
 // 16 as in global memory so that its middle moves in 16-byte words; nothing
 // outside the segment's bytes is read.
@@ -412,7 +406,7 @@ __global__ void __launch_bounds__(kWThreads) weights_i8_kernel(const WeightArgs 
                 for (uint32_t i = 0; i < 32; i++) {
                     if (i >= n) break;
                     if (pass == 0) m = max(m, abs_bits(y[i]));
-                    else q[e0 + u * 32 + i] = (int8_t)quant_exact(y[i], rs);
+                    else q[e0 + u * 32 + i] = (int8_t)quant1(y[i], rs);
                 }
             }
         }
@@ -424,8 +418,132 @@ __global__ void __launch_bounds__(kWThreads) weights_i8_kernel(const WeightArgs 
     if (threadIdx.x == 0) a.scale[row] = rs.scale;
 }
 
+// The same for rows that fit: a CTA walks groups of rows (back to back in memory),
+// copies the next group's bytes while it works on this one's, and each thread
+// keeps the U units it decodes in registers from the maximum to the rounding. tpr
+// threads (whole warps) a row.
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n"
+                 ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void stage_async(uint8_t* sm, const uint8_t* src, uint32_t n) {
+    const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(src) & 15u);
+    const uint32_t head = min(n, (16u - off) & 15u), vecs = (n - head) / 16, tail = n - head - vecs * 16;
+    uint8_t* dst = sm + off;
+    for (uint32_t i = threadIdx.x; i < vecs; i += blockDim.x) copy16(dst + head + i * 16, src + head + i * 16);
+    for (uint32_t i = threadIdx.x; i < head + tail; i += blockDim.x) {
+        const uint32_t at = i < head ? i : head + vecs * 16 + (i - head);
+        dst[at] = src[at];
+    }
+}
+
+template <uint32_t T, uint32_t U>
+__global__ void __launch_bounds__(512, U == 1 ? 2 : 1) weights_i8_rows_kernel(const WeightArgs a, uint32_t tpr, uint32_t buf) {
+    extern __shared__ __align__(16) uint8_t sm[];    // two buffers of `buf` bytes
+    __shared__ uint32_t red[16];
+    const uint32_t rows = blockDim.x / tpr, r = threadIdx.x / tpr, t = threadIdx.x - r * tpr;
+    const uint32_t units = (a.cols + 31) / 32, groups = (a.rows + rows - 1) / rows;
+    pdl_trigger();
+    pdl_wait();
+    auto stage = [&](uint32_t g, uint32_t turn) {
+        const uint64_t row0 = (uint64_t)g * rows;
+        const uint32_t n = (uint32_t)min((uint64_t)rows, a.rows - row0);
+        stage_async(sm + (turn & 1u) * buf, a.raw + row0 * a.row_bytes, (uint32_t)(n * a.row_bytes));
+    };
+    stage(blockIdx.x, 0);
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+    for (uint32_t g = blockIdx.x, turn = 0; g < groups; g += gridDim.x, turn++) {
+        if (g + gridDim.x < groups) stage(g + gridDim.x, turn + 1);
+        asm volatile("cp.async.commit_group;\ncp.async.wait_group 1;\n" ::: "memory");
+        __syncthreads();
+        const uint64_t row = (uint64_t)g * rows + r;
+        const uint8_t* p = sm + (turn & 1u) * buf +
+                           (uint32_t)(reinterpret_cast<uintptr_t>(a.raw + (uint64_t)g * rows * a.row_bytes) & 15u);
+        float y[U][32], top = 0.f;
+        if (row < a.rows) {
+#pragma unroll
+            for (uint32_t j = 0; j < U; j++) {
+                const uint32_t u = t + j * tpr;
+                if (u >= units) break;
+                unit_weights<T>(p + r * (uint32_t)a.row_bytes, u, y[j]);
+                const uint32_t left = a.cols - u * 32;
+#pragma unroll
+                for (uint32_t i = 0; i < 32; i++) {
+                    if ((T == GGML_TYPE_F32 || T == GGML_TYPE_F16) && i >= left) y[j][i] = 0.f;   // a short last unit
+                    top = max_abs(top, y[j][i]);
+                }
+            }
+        }
+        uint32_t m = __reduce_max_sync(0xffffffffu, abs_bits(top));
+        if ((threadIdx.x & 31u) == 0) red[threadIdx.x >> 5] = m;
+        __syncthreads();                             // (and every thread has read this buffer)
+        if (row >= a.rows) continue;
+        m = 0;
+        for (uint32_t i = 0; i < tpr / 32; i++) m = max(m, red[r * (tpr / 32) + i]);
+        const RowScale rs = row_scale(__uint_as_float(m));
+        int8_t* q = a.q + row * a.ld_q;
+        const bool odd = t & 1u;
+#pragma unroll
+        for (uint32_t j = 0; j < U; j++) {
+            const uint32_t u = t + j * tpr;
+            uint32_t w[8];
+            if (!rs.zero && !rs.tiny) {
+#pragma unroll
+                for (uint32_t i = 0; i < 8; i++)
+                    w[i] = low_bytes(fmaf(y[j][4 * i], rs.inv, kRound), fmaf(y[j][4 * i + 1], rs.inv, kRound),
+                                     fmaf(y[j][4 * i + 2], rs.inv, kRound), fmaf(y[j][4 * i + 3], rs.inv, kRound));
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < 8; i++) {
+                    w[i] = 0;
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; k++) w[i] |= ((uint32_t)quant1(y[j][4 * i + k], rs) & 0xFFu) << (8 * k);
+                }
+            }
+            // 32 bytes a unit: the even lane stores the first 16 of its own unit, the
+            // odd one the second 16 of that, then the same for the odd lane's unit,
+            // so that a store covers whole 32-byte sectors (lanes without a unit take part)
+            uint32_t s1[4], s2[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                const uint32_t give = odd ? w[i] : w[4 + i];
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, give, 1);
+                s1[i] = odd ? got : w[i];
+                s2[i] = odd ? w[4 + i] : got;
+            }
+            const uint32_t e1 = (u & ~1u) * 32 + (odd ? 16 : 0), e2 = e1 + 32;
+            if (e1 + 16 <= a.cols) *reinterpret_cast<uint4*>(q + e1) = make_uint4(s1[0], s1[1], s1[2], s1[3]);
+            else
+                for (uint32_t i = 0; i < 16; i++)
+                    if (e1 + i < a.cols) q[e1 + i] = (int8_t)(s1[i >> 2] >> (8 * (i & 3u)));
+            if (e2 + 16 <= a.cols) *reinterpret_cast<uint4*>(q + e2) = make_uint4(s2[0], s2[1], s2[2], s2[3]);
+            else
+                for (uint32_t i = 0; i < 16; i++)
+                    if (e2 + i < a.cols) q[e2 + i] = (int8_t)(s2[i >> 2] >> (8 * (i & 3u)));
+        }
+        if (t == 0) a.scale[row] = rs.scale;
+    }
+}
+
 template <uint32_t T>
 bool launch_weights(const WeightArgs& a, cudaStream_t st) {
+    // rows of up to 1024 units whose int8 rows start on 16 bytes
+    const uint32_t units = (a.cols + 31) / 32, U = units <= 512 ? 1 : 2, tpr = (units + 32 * U - 1) / (32 * U) * 32;
+    if (tpr <= 512 && i8_aligned(a.q, 16) && a.ld_q % 16 == 0 && a.row_bytes <= kWRow) {
+        uint32_t rows = tpr < 256 ? 256 / tpr : 1;   // about 256 threads a CTA
+        while (rows > 1 && rows * a.row_bytes > kWRow / 4) rows--;
+        const uint32_t buf = ((uint32_t)(rows * a.row_bytes) + kWSlack + 15u) & ~15u, smem = 2 * buf;
+        auto* kernel = U == 1 ? weights_i8_rows_kernel<T, 1> : weights_i8_rows_kernel<T, 2>;
+        if (smem > 48 * 1024 &&
+            !LM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * (kWRow + kWSlack + 16)))))
+            return false;
+        // CTAs that run at once: by threads and shared memory, two by registers at 512 threads
+        uint32_t occ = (200 * 1024) / (smem + 1024);
+        if (occ * rows * tpr > 1024) occ = 1024 / (rows * tpr);
+        if (occ < 1) occ = 1;
+        const uint32_t groups = (a.rows + rows - 1) / rows, most = i8_sms() * occ;
+        return LM_CUDA(launch_k(kernel, dim3(groups < most ? groups : most), dim3(rows * tpr), smem, st, a, tpr, buf));
+    }
     const uint32_t smem = (uint32_t)(a.row_bytes < kWSeg ? a.row_bytes : kWSeg) + kWSlack;
     if (smem > 48 * 1024 &&
         !LM_CUDA(cudaFuncSetAttribute(weights_i8_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kWSeg + kWSlack))))
@@ -464,22 +582,23 @@ bool align_ok(const char* who, const void* const* ptrs, int n, size_t bytes) {
 }
 
 // CTAs of a kernel that walks `rows` rows, `per` at a time: as many as run at
-// once, and no more than there are rows.
+// once, and no more than there are rows. occupancy: CTAs an SM by warps of a CTA,
+// looked up once.
 template <typename K>
-uint32_t walkers(std::atomic<uint32_t>& memo, K* kernel, uint32_t threads, uint64_t rows, uint32_t per) {
-    uint32_t n = memo.load(std::memory_order_relaxed);
-    if (n == 0) {
-        int dev = 0, sms = 0, occ = 0;
-        if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kernel, (int)threads, 0) != cudaSuccess || sms * occ <= 0) {
+uint32_t walkers(std::atomic<int>* occupancy, K* kernel, uint32_t threads, uint64_t rows, uint32_t per) {
+    const uint32_t sms = i8_sms();
+    const uint64_t want = (rows + per - 1) / per;
+    if (want <= sms) return (uint32_t)want;
+    std::atomic<int>& memo = occupancy[threads / 32];
+    int occ = memo.load(std::memory_order_relaxed);
+    if (occ == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kernel, (int)threads, 0) != cudaSuccess || occ < 1) {
             cudaGetLastError();
-            sms = 148;
             occ = 1;
         }
-        n = (uint32_t)(sms * occ);
-        memo.store(n, std::memory_order_relaxed);
+        memo.store(occ, std::memory_order_relaxed);
     }
-    const uint64_t want = (rows + per - 1) / per;
+    const uint64_t n = (uint64_t)sms * occ;
     return (uint32_t)(want < n ? want : n);
 }
 template <typename T> bool vec_rows(const void* p, uint64_t ld) {
@@ -489,52 +608,62 @@ template <typename T> bool vec_q(const int8_t* q, uint64_t ld) {
     return i8_aligned(q, vec_elems<T>()) && ld % vec_elems<T>() == 0;
 }
 
-template <typename T, uint32_t G, uint32_t V, bool RESID>
-bool launch_norm_rows(const NormArgs& a, cudaStream_t st) {
-    static std::atomic<uint32_t> memo{0};
-    constexpr uint32_t threads = G == 32 ? 32 * kWarpRows : G, per = G == 32 ? kWarpRows : 1;
-    const uint32_t grid = walkers(memo, norm_i8_rows_kernel<T, G, V, RESID>, threads, a.rows, per);
-    return LM_CUDA(launch_k(norm_i8_rows_kernel<T, G, V, RESID>, dim3(grid), dim3(threads), 0, st, a));
+// How a launch spreads its rows: a warp each, or CTAs of `threads`.
+struct RowShape {
+    uint32_t threads, per;
+};
+
+template <typename T, bool RESID, bool WARP, uint32_t V>
+bool launch_norm_rows(const NormArgs& a, const RowShape& r, cudaStream_t st) {
+    static std::atomic<int> occupancy[33];
+    const uint32_t grid = walkers(occupancy, norm_i8_rows_kernel<T, RESID, WARP, V>, r.threads, a.rows, r.per);
+    return LM_CUDA(launch_k(norm_i8_rows_kernel<T, RESID, WARP, V>, dim3(grid), dim3(r.threads), 0, st, a));
 }
-template <typename T, uint32_t G, uint32_t V>
-bool launch_norm_rows(const NormArgs& a, cudaStream_t st) {
-    return a.resid ? launch_norm_rows<T, G, V, true>(a, st) : launch_norm_rows<T, G, V, false>(a, st);
-}
-template <typename T, uint32_t ACT, uint32_t G, uint32_t V>
-bool launch_glu_rows(const GluArgs& a, cudaStream_t st) {
-    static std::atomic<uint32_t> memo{0}, memo1{0};
-    constexpr uint32_t threads = G == 32 ? 32 * kWarpRows : G, per = G == 32 ? kWarpRows : 1;
-    if (a.up) {
-        const uint32_t grid = walkers(memo, glu_i8_rows_kernel<T, ACT, true, G, V>, threads, a.rows, per);
-        return LM_CUDA(launch_k(glu_i8_rows_kernel<T, ACT, true, G, V>, dim3(grid), dim3(threads), 0, st, a));
-    }
-    const uint32_t grid = walkers(memo1, glu_i8_rows_kernel<T, ACT, false, G, V>, threads, a.rows, per);
-    return LM_CUDA(launch_k(glu_i8_rows_kernel<T, ACT, false, G, V>, dim3(grid), dim3(threads), 0, st, a));
+template <typename T, uint32_t ACT, bool UP, bool WARP, uint32_t V>
+bool launch_glu_rows(const GluArgs& a, const RowShape& r, cudaStream_t st) {
+    static std::atomic<int> occupancy[33];
+    const uint32_t grid = walkers(occupancy, glu_i8_rows_kernel<T, ACT, UP, WARP, V>, r.threads, a.rows, r.per);
+    return LM_CUDA(launch_k(glu_i8_rows_kernel<T, ACT, UP, WARP, V>, dim3(grid), dim3(r.threads), 0, st, a));
 }
 
-// Threads a row and vectors a thread. Many short rows: a warp each; otherwise the
-// smallest CTA that holds the row in up to 4 vectors a thread. Rows past 4096
-// vectors, and pitches or bases that are not whole vectors, take the two-pass
-// kernel.
-#define LM_I8_ROWS(LAUNCH, ...)                                              \
-    do {                                                                     \
-        const uint32_t nv = (a.cols + vec_elems<T>() - 1) / vec_elems<T>();  \
-        if (a.rows >= 1024 && nv <= 32) return LAUNCH<__VA_ARGS__, 32, 1>(a, st);  \
-        if (a.rows >= 1024 && nv <= 64) return LAUNCH<__VA_ARGS__, 32, 2>(a, st);  \
-        if (a.rows >= 1024 && nv <= 128) return LAUNCH<__VA_ARGS__, 32, 4>(a, st); \
-        if (nv <= 128) return LAUNCH<__VA_ARGS__, 128, 1>(a, st);            \
-        if (nv <= 256) return LAUNCH<__VA_ARGS__, 128, 2>(a, st);            \
-        if (nv <= 512) return LAUNCH<__VA_ARGS__, 256, 2>(a, st);            \
-        if (nv <= 1024) return LAUNCH<__VA_ARGS__, 512, 2>(a, st);           \
-        if (nv <= 1536) return LAUNCH<__VA_ARGS__, 512, 3>(a, st);           \
-        if (nv <= 2048) return LAUNCH<__VA_ARGS__, 512, 4>(a, st);           \
-        if (nv <= 4096) return LAUNCH<__VA_ARGS__, 1024, 4>(a, st);          \
+// Calls LAUNCH for the shape that fits rows of `cols` elements; falls through
+// when no shape does.
+#define LM_I8_ROWS(LAUNCH, ...)                                                             \
+    do {                                                                                    \
+        const uint32_t nv = (a.cols + vec_elems<T>() - 1) / vec_elems<T>();                 \
+        int tv = getenv("I8_V") ? atoi(getenv("I8_V")) : 0;                          \
+        const uint32_t V = tv ? tv : rows_vectors(a.rows, nv);                                   \
+        if (V % 10 == 0) break;                                                             \
+        const RowShape w = {32 * kWarpRows, kWarpRows}, r = {((nv + V % 10 - 1) / (V % 10) + 31) / 32 * 32, 1}; \
+        if (V > 10 ? nv > 32 * (V - 10) : r.threads > (V > 1 ? 512u : 1024u)) break;       \
+        switch (V) {                                                                        \
+        case 11: return LAUNCH<__VA_ARGS__, true, 1>(a, w, st);                             \
+        case 12: return LAUNCH<__VA_ARGS__, true, 2>(a, w, st);                             \
+        case 14: return LAUNCH<__VA_ARGS__, true, 4>(a, w, st);                             \
+        case 1: return LAUNCH<__VA_ARGS__, false, 1>(a, r, st);                             \
+        case 2: return LAUNCH<__VA_ARGS__, false, 2>(a, r, st);                             \
+        case 3: return LAUNCH<__VA_ARGS__, false, 3>(a, r, st);                             \
+        case 4: return LAUNCH<__VA_ARGS__, false, 4>(a, r, st);                             \
+        case 8: return LAUNCH<__VA_ARGS__, false, 8>(a, r, st);                             \
+        }                                                                                   \
     } while (0)
+
+uint32_t rows_vectors(uint32_t rows, uint32_t nv) {
+    if (rows >= 1024 && nv <= 32) return 11;
+    if (rows >= 1024 && nv <= 64) return 12;
+    if (rows >= 1024 && nv <= 128) return 14;
+    if (nv <= 128) return 1;
+    if (nv <= 1024) return 2;
+    if (nv <= 2048) return 4;
+    return nv <= 4096 ? 8 : 0;
+}
 
 template <typename T, uint32_t ACT>
 bool launch_glu_act(const GluArgs& a, cudaStream_t st) {
-    if (vec_rows<T>(a.gate, a.ld_gate) && vec_rows<T>(a.up, a.ld_up) && vec_q<T>(a.q, a.ld_q))
-        LM_I8_ROWS(launch_glu_rows, T, ACT);
+    if (vec_rows<T>(a.gate, a.ld_gate) && vec_rows<T>(a.up, a.ld_up) && vec_q<T>(a.q, a.ld_q)) {
+        if (a.up) LM_I8_ROWS(launch_glu_rows, T, ACT, true);
+        else LM_I8_ROWS(launch_glu_rows, T, ACT, false);
+    }
     glu_i8_kernel<T, ACT><<<a.rows, 256, 0, st>>>(a);
     return LM_CUDA(cudaGetLastError());
 }
@@ -547,8 +676,10 @@ bool launch_glu(const GluArgs& a, cudaStream_t st) {
 template <typename T>
 bool launch_norm(const NormArgs& a, cudaStream_t st) {
     if (vec_rows<T>(a.x, a.ld_x) && vec_rows<T>(a.resid, a.ld_resid) && vec_rows<T>(a.sum, a.ld_sum) &&
-        i8_aligned(a.w, 16) && vec_q<T>(a.q, a.ld_q))
-        LM_I8_ROWS(launch_norm_rows, T);
+        i8_aligned(a.w, 16) && vec_q<T>(a.q, a.ld_q)) {
+        if (a.resid) LM_I8_ROWS(launch_norm_rows, T, true);
+        else LM_I8_ROWS(launch_norm_rows, T, false);
+    }
     norm_i8_kernel<T><<<a.rows, 256, 0, st>>>(a);
     return LM_CUDA(cudaGetLastError());
 }

@@ -257,12 +257,12 @@ def _weights_call(gpu, t, raw, rows, cols, q, scale):
 
 
 def _want_weights(w):
-    """Exact: the f32 scale, then the quotient of two f32 numbers in 64 bits,
-    which tells every quotient from a tie."""
-    s = (w.abs().amax(dim=1).double() / 127).float()
-    d = torch.where(s > 0, s, torch.ones_like(s)).double()
-    q = torch.round(w.double() / d[:, None]) * (s > 0)[:, None]
-    return q.to(torch.int8), s
+    """Exact: the f32 scale and reciprocal, then the product of two f32 numbers
+    in 64 bits, which holds it whole."""
+    top = w.abs().amax(dim=1).double()
+    s = (top / 127).float()
+    inv = torch.where(top > 0, 127 / top, torch.zeros_like(top)).float().double()
+    return torch.round(w.double() * inv[:, None]).to(torch.int8), s
 
 
 @pytest.mark.parametrize("t", [0, 1, 2, 3, 6, 8, 12, 13, 14])
@@ -326,7 +326,7 @@ def test_weights_special_scales(gpu, orc, golden, t):
     assert torch.isnan(scale[~fine]).all() and torch.all(q.t[~fine] == 0)
     want_q, want_s = _want_weights(w[fine])
     assert torch.equal(scale[fine], want_s)
-    normal = want_s > 1.2e-38                      # below, scales are subnormal: as in test_glu_extreme_rows
+    normal = want_s > 1.2e-38                      # below, q is w / scale and scales are subnormal: as in test_glu_extreme_rows
     assert torch.equal(q.t[fine][normal], want_q[normal])
     rest, s = q.t[fine][~normal].double(), want_s[~normal].double()
     assert torch.all((rest * s[:, None] - w[fine][~normal].double()).abs() <= s[:, None] / 2 + 127 * 2.0 ** -150)
