@@ -91,7 +91,7 @@ __device__ __forceinline__ uint32_t abs_bits(float y) { return __float_as_uint(y
 // max(m, |y|), NaN when either is: one instruction an element.
 __device__ __forceinline__ float max_abs(float m, float y) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(m), "f"(fabsf(y)));
+    asm("{\n .reg .f32 t;\n abs.f32 t, %2;\n max.NaN.f32 %0, %1, t;\n}\n" : "=f"(r) : "f"(m), "f"(y));
     return r;
 }
 
@@ -99,27 +99,30 @@ __device__ __forceinline__ float max_abs(float m, float y) {
 // integer (ties to even), in the low mantissa bits: the low byte is the int8.
 constexpr float kRound = 12582912.0f;
 
-// The scale of a row whose largest magnitude has these bits, and how its
-// elements become integers.
+// How the elements of a row with this largest magnitude become integers, and
+// the row's scale (a division that only one thread of a row needs).
 struct RowScale {
-    float scale, inv;
-    bool tiny, zero;
+    float amax, inv;
+    bool bad, tiny;            // NaN or infinity in the row; 127 / amax overflows (or the row is zero)
+    __device__ __forceinline__ float scale() const { return bad ? NAN : __fdiv_rn(amax, 127.0f); }
+    __device__ __forceinline__ bool plain() const { return !bad && !tiny; }
 };
 __device__ __forceinline__ RowScale row_scale(float amax) {
     RowScale r;
-    const bool bad = !(amax < INFINITY);
-    r.scale = bad ? NAN : __fdiv_rn(amax, 127.0f);
-    // below 1.5e-36 the scale is subnormal or 127 / max overflows
+    r.amax = amax;
+    r.bad = !(amax < INFINITY);
     r.tiny = amax < 1.5e-36f;
-    r.zero = bad || r.scale == 0.0f;
-    r.inv = r.tiny || bad ? 0.0f : __fdiv_rn(127.0f, amax);
+    r.inv = __fdiv_rn(127.0f, amax);
     return r;
 }
-// One element of a row.
+// One element of a row; out of line where the row is not plain.
+inline __device__ __noinline__ int quant_odd(float y, const RowScale r) {
+    const float s = r.scale();
+    if (r.bad || s == 0.0f) return 0;
+    return max(-127, min(127, __float2int_rn(__fdiv_rn(y, s))));
+}
 __device__ __forceinline__ int quant1(float y, const RowScale& r) {
-    if (r.zero) return 0;
-    if (r.tiny) return max(-127, min(127, __float2int_rn(__fdiv_rn(y, r.scale))));
-    return (int)(int8_t)__float_as_uint(fmaf(y, r.inv, kRound));
+    return r.plain() ? (int)(int8_t)__float_as_uint(fmaf(y, r.inv, kRound)) : quant_odd(y, r);
 }
 
 // Block-wide maximum of unsigned integers and sum of floats; every thread gets
@@ -145,8 +148,9 @@ __device__ __forceinline__ void block_max_sum(uint32_t& m, float& s, uint32_t* r
 
 // ---------------------------------------------------------------- rows in registers
 //
-// A row of 16-byte vectors spread over G threads (a warp, or a whole CTA), up to
-// V vectors a thread, vector j of thread t at t + j G.
+// A row in pieces of E elements (16 bytes, or one element where pitches or bases
+// are not whole 16 bytes) spread over G threads (a warp, or a whole CTA), up to V
+// pieces a thread, piece j of thread t at t + j G.
 
 template <typename T> constexpr uint32_t vec_elems() { return 16 / sizeof(T); }
 
@@ -185,31 +189,49 @@ __device__ __forceinline__ uint4 f32_to_vec(const float* f) {
     else
         return make_uint4(pack2(f[0], f[1], T()), pack2(f[2], f[3], T()), pack2(f[4], f[5], T()), pack2(f[6], f[7], T()));
 }
-// Elements [at, at + vec_elems) of a row; past the row's end zeros, read one by one.
-template <typename T>
-__device__ __forceinline__ uint4 load_vec(const T* row, uint32_t at, uint32_t cols) {
-    constexpr uint32_t E = vec_elems<T>();
-    if (at + E <= cols) return *reinterpret_cast<const uint4*>(row + at);
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (at < cols) {
-        T e[E];
-        *reinterpret_cast<uint4*>(e) = v;
-        for (uint32_t i = 0; i < E; i++)
-            if (at + i < cols) e[i] = row[at + i];
-        v = *reinterpret_cast<uint4*>(e);
+// A piece as it lies in memory.
+template <typename T, uint32_t E> struct Piece { uint4 v; };
+template <typename T> struct Piece<T, 1> { T v; };
+
+// Elements [at, at + E) of a row; past the row's end zeros, and nothing is read there.
+template <typename T, uint32_t E>
+__device__ __forceinline__ void load_piece(Piece<T, E>& p, const T* row, uint32_t at, uint32_t cols) {
+    if constexpr (E == 1) {
+        p.v = at < cols ? row[at] : from_f32<T>(0.f);
+    } else {
+        if (at + E <= cols) {
+            p.v = *reinterpret_cast<const uint4*>(row + at);
+            return;
+        }
+        p.v = make_uint4(0, 0, 0, 0);
+        if (at < cols) {
+            T e[E];
+            *reinterpret_cast<uint4*>(e) = p.v;
+            for (uint32_t i = 0; i < E; i++)
+                if (at + i < cols) e[i] = row[at + i];
+            p.v = *reinterpret_cast<uint4*>(e);
+        }
     }
-    return v;
 }
-template <typename T>
-__device__ __forceinline__ void store_vec(T* row, uint32_t at, uint32_t cols, const uint4& v) {
-    constexpr uint32_t E = vec_elems<T>();
-    if (at + E <= cols) {
-        *reinterpret_cast<uint4*>(row + at) = v;
-        return;
+template <typename T, uint32_t E>
+__device__ __forceinline__ void piece_to_f32(const Piece<T, E>& p, float* f) {
+    if constexpr (E == 1) f[0] = to_f32(p.v);
+    else vec_to_f32<T>(p.v, f);
+}
+template <typename T, uint32_t E>
+__device__ __forceinline__ void store_piece(T* row, uint32_t at, uint32_t cols, const float* f) {
+    if constexpr (E == 1) {
+        if (at < cols) row[at] = from_f32<T>(f[0]);
+    } else {
+        const uint4 v = f32_to_vec<T>(f);
+        if (at + E <= cols) {
+            *reinterpret_cast<uint4*>(row + at) = v;
+            return;
+        }
+        const T* e = reinterpret_cast<const T*>(&v);
+        for (uint32_t i = 0; i < E; i++)
+            if (at + i < cols) row[at + i] = e[i];
     }
-    const T* e = reinterpret_cast<const T*>(&v);
-    for (uint32_t i = 0; i < E; i++)
-        if (at + i < cols) row[at + i] = e[i];
 }
 
 __device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d) {
@@ -219,31 +241,34 @@ __device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d
 }
 
 // E values of a row, times f (127 / max, or what maps onto it), to int8 at q + at.
-// `r` decides for rows whose scale is zero, not finite or subnormal; y maps a
-// value to what r.scale stands for.
+// Rows that are not plain go by y(value), what the row's scale is of.
 template <uint32_t E, typename Y>
 __device__ __forceinline__ void store_quant(int8_t* q, uint32_t at, uint32_t cols, const float* v, float f,
-                                            const RowScale& r, Y y) {
-    uint32_t w[E / 4];
-    if (!r.tiny && !r.zero) {
-#pragma unroll
-        for (uint32_t i = 0; i < E / 4; i++)
-            w[i] = low_bytes(fmaf(v[4 * i], f, kRound), fmaf(v[4 * i + 1], f, kRound), fmaf(v[4 * i + 2], f, kRound),
-                             fmaf(v[4 * i + 3], f, kRound));
+                                            const RowScale& r, bool plain, Y y) {
+    if constexpr (E == 1) {
+        if (at < cols) q[at] = plain ? (int8_t)__float_as_uint(fmaf(v[0], f, kRound)) : (int8_t)quant_odd(y(v[0]), r);
     } else {
+        uint32_t w[E / 4];
+        if (plain) {
 #pragma unroll
-        for (uint32_t i = 0; i < E / 4; i++) {
-            w[i] = 0;
+            for (uint32_t i = 0; i < E / 4; i++)
+                w[i] = low_bytes(fmaf(v[4 * i], f, kRound), fmaf(v[4 * i + 1], f, kRound), fmaf(v[4 * i + 2], f, kRound),
+                                 fmaf(v[4 * i + 3], f, kRound));
+        } else {
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++) w[i] |= ((uint32_t)quant1(y(v[4 * i + j]), r) & 0xFFu) << (8 * j);
+            for (uint32_t i = 0; i < E / 4; i++) {
+                w[i] = 0;
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) w[i] |= ((uint32_t)quant_odd(y(v[4 * i + j]), r) & 0xFFu) << (8 * j);
+            }
         }
-    }
-    if (at + E <= cols) {
-        if constexpr (E == 8) *reinterpret_cast<uint2*>(q + at) = make_uint2(w[0], w[1]);
-        else *reinterpret_cast<uint32_t*>(q + at) = w[0];
-    } else {
-        for (uint32_t i = 0; i < E; i++)
-            if (at + i < cols) q[at + i] = (int8_t)(w[i >> 2] >> (8 * (i & 3u)));
+        if (at + E <= cols) {
+            if constexpr (E == 8) *reinterpret_cast<uint2*>(q + at) = make_uint2(w[0], w[1]);
+            else *reinterpret_cast<uint32_t*>(q + at) = w[0];
+        } else {
+            for (uint32_t i = 0; i < E; i++)
+                if (at + i < cols) q[at + i] = (int8_t)(w[i >> 2] >> (8 * (i & 3u)));
+        }
     }
 }
 

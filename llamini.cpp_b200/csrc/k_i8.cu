@@ -15,8 +15,8 @@ namespace lm {
 namespace {
 
 constexpr uint32_t kWarpRows = 8;          // rows at a time of a CTA whose warps have one each
-// The most threads of a CTA that keeps up to V vectors a thread in registers.
-template <bool WARP, uint32_t V> constexpr uint32_t rows_threads() { return WARP ? 32 * kWarpRows : V > 1 ? 512 : 1024; }
+// The most threads of a CTA that keeps up to N elements a thread in registers.
+template <bool WARP, uint32_t N> constexpr uint32_t rows_threads() { return WARP ? 32 * kWarpRows : N > 8 ? 512 : 1024; }
 
 // ---------------------------------------------------------------- norm
 
@@ -58,15 +58,14 @@ __global__ void __launch_bounds__(256) norm_i8_kernel(const NormArgs a) {
         if (o) o[i] = from_f32<T>(h);
         a.q[row * a.ld_q + i] = (int8_t)quant1(h * a.w[i] * rstd, s);
     }
-    if (threadIdx.x == 0) a.scale[row] = s.scale;
+    if (threadIdx.x == 0) a.scale[row] = s.scale();
 }
 
 // The same with a row in the registers of G threads (V vectors each), read once:
 // h w of every element is kept from the first pass to the second. CTAs walk the
 // rows with w in registers and the next row's loads in flight.
-template <typename T, bool RESID, bool WARP, uint32_t V>
-__global__ void __launch_bounds__(rows_threads<WARP, V>()) norm_i8_rows_kernel(const NormArgs a) {
-    constexpr uint32_t E = vec_elems<T>();
+template <typename T, bool RESID, bool WARP, uint32_t E, uint32_t V>
+__global__ void __launch_bounds__(rows_threads<WARP, V * E>()) norm_i8_rows_kernel(const NormArgs a) {
     constexpr uint32_t R = WARP ? kWarpRows : 1;     // rows of a CTA at a time
     constexpr bool AHEAD = V * E <= 32;              // the next row's vectors fit the registers too
     __shared__ uint32_t red[WARP ? 1 : 128];
@@ -79,18 +78,18 @@ __global__ void __launch_bounds__(rows_threads<WARP, V>()) norm_i8_rows_kernel(c
 #pragma unroll
     for (uint32_t j = 0; j < V; j++)
 #pragma unroll
-        for (uint32_t i = 0; i < E; i += 4) {
-            const uint4 v = load_vec<float>(a.w, (t + j * G) * E + i, a.cols);
-            vec_to_f32<float>(v, &w[j][i]);
+        for (uint32_t i = 0; i < E; i++) {
+            const uint32_t at = (t + j * G) * E + i;
+            w[j][i] = at < a.cols ? a.w[at] : 0.f;
         }
-    uint4 x[V], r[V];
+    Piece<T, E> x[V], r[V];
     auto load = [&](uint64_t at) {
         const T* px = static_cast<const T*>(a.x) + at * a.ld_x;
         const T* pr = static_cast<const T*>(a.resid) + at * a.ld_resid;
 #pragma unroll
         for (uint32_t j = 0; j < V; j++) {
-            x[j] = load_vec<T>(px, (t + j * G) * E, a.cols);
-            if (RESID) r[j] = load_vec<T>(pr, (t + j * G) * E, a.cols);
+            load_piece<T, E>(x[j], px, (t + j * G) * E, a.cols);
+            if (RESID) load_piece<T, E>(r[j], pr, (t + j * G) * E, a.cols);
         }
     };
     if (AHEAD && row < a.rows) load(row);
@@ -101,14 +100,14 @@ __global__ void __launch_bounds__(rows_threads<WARP, V>()) norm_i8_rows_kernel(c
         T* o = a.sum ? static_cast<T*>(a.sum) + row * a.ld_sum : nullptr;
 #pragma unroll
         for (uint32_t j = 0; j < V; j++) {
-            vec_to_f32<T>(x[j], hw[j]);
+            piece_to_f32<T, E>(x[j], hw[j]);
             if (RESID) {
                 float f[E];
-                vec_to_f32<T>(r[j], f);
+                piece_to_f32<T, E>(r[j], f);
 #pragma unroll
                 for (uint32_t i = 0; i < E; i++) hw[j][i] += f[i];
             }
-            if (o) store_vec<T>(o, (t + j * G) * E, a.cols, f32_to_vec<T>(hw[j]));
+            if (o) store_piece<T, E>(o, (t + j * G) * E, a.cols, hw[j]);
 #pragma unroll
             for (uint32_t i = 0; i < E; i++) {
                 ss = fmaf(hw[j][i], hw[j][i], ss);
@@ -120,13 +119,13 @@ __global__ void __launch_bounds__(rows_threads<WARP, V>()) norm_i8_rows_kernel(c
         uint32_t m = abs_bits(top);
         row_max_sum<WARP>(m, ss, red, turn);
         const float rstd = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
-        RowScale s = row_scale(__uint_as_float(m) * rstd);
+        const RowScale s = row_scale(__uint_as_float(m) * rstd);
         const float f = rstd * s.inv;
-        s.tiny |= !(f < INFINITY);
+        const bool plain = s.plain() && f < INFINITY;
 #pragma unroll
         for (uint32_t j = 0; j < V; j++)
-            store_quant<E>(a.q + row * a.ld_q, (t + j * G) * E, a.cols, hw[j], f, s, [&](float v) { return v * rstd; });
-        if (t == 0) a.scale[row] = s.scale;
+            store_quant<E>(a.q + row * a.ld_q, (t + j * G) * E, a.cols, hw[j], f, s, plain, [&](float v) { return v * rstd; });
+        if (t == 0) a.scale[row] = s.scale();
     }
 }
 
@@ -141,16 +140,26 @@ struct GluArgs {
     uint32_t rows, cols, act;
 };
 
-// The activations of model.c:14-25 (and gpt2.c's gelu), in f32. GELU's (1 +
-// tanh z) / 2 is 1 / (1 + exp(-2 z)), which does not cancel for negative z and
-// costs one exponential. The quotients use the approximate division (2 ulp): the
-// result is rounded to 8 bits.
+// The activations of model.c:14-25 (and gpt2.c's gelu), in f32, as x / (1 +
+// exp(-z)): SiLU's z is x; GELU's (1 + tanh u) / 2 is 1 / (1 + exp(-2 u)), which
+// does not cancel for negative u. exp(-z) is 2^(-z log2 e) with the factor folded
+// into z's constants: its argument's rounding leaves a relative error of up to
+// |z| 2^-24, next to the 2^-22 of the two approximate instructions, where the
+// result is rounded to 8 bits. 26 instructions an element became 14 (4096 x 11008
+// bf16: 58 us with expf and an exact division).
+__device__ __forceinline__ float sigmoid_of(float minus_z_log2e) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(e) : "f"(minus_z_log2e));
+    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(1.0f + e));
+    return r;
+}
 template <uint32_t ACT>
 __device__ __forceinline__ float activate(float x) {
-    if (ACT == ACT_SILU) return __fdividef(x, 1.0f + expf(-x));
+    constexpr float log2e = 1.4426950408889634f;
+    if (ACT == ACT_SILU) return x * sigmoid_of(x * -log2e);
     if (ACT == ACT_GELU) {
-        const float k0 = 2.0f * 0.79788456080286535587989211986876f;
-        return __fdividef(x, 1.0f + expf(-k0 * x * (1.0f + 0.044715f * x * x)));
+        constexpr float k = -2.0f * 0.79788456080286535587989211986876f * log2e;
+        return x * sigmoid_of(x * fmaf(0.044715f * k, x * x, k));
     }
     return x;
 }
@@ -169,14 +178,13 @@ __global__ void __launch_bounds__(256) glu_i8_kernel(const GluArgs a) {
     const RowScale s = row_scale(__uint_as_float(m));
     for (uint32_t i = threadIdx.x; i < a.cols; i += blockDim.x)
         a.q[row * a.ld_q + i] = (int8_t)quant1(activate<ACT>(to_f32(g[i])) * (u ? to_f32(u[i]) : 1.f), s);
-    if (threadIdx.x == 0) a.scale[row] = s.scale;
+    if (threadIdx.x == 0) a.scale[row] = s.scale();
 }
 
 // The same with a row's values in the registers of G threads, read and
 // activated once; the next row's loads are in flight meanwhile.
-template <typename T, uint32_t ACT, bool UP, bool WARP, uint32_t V>
-__global__ void __launch_bounds__(rows_threads<WARP, V>()) glu_i8_rows_kernel(const GluArgs a) {
-    constexpr uint32_t E = vec_elems<T>();
+template <typename T, uint32_t ACT, bool UP, bool WARP, uint32_t E, uint32_t V>
+__global__ void __launch_bounds__(rows_threads<WARP, V * E>()) glu_i8_rows_kernel(const GluArgs a) {
     constexpr uint32_t R = WARP ? kWarpRows : 1;
     constexpr bool AHEAD = V * E <= 32;
     __shared__ uint32_t red[WARP ? 1 : 128];
@@ -185,14 +193,14 @@ __global__ void __launch_bounds__(rows_threads<WARP, V>()) glu_i8_rows_kernel(co
     const uint64_t step = (uint64_t)gridDim.x * R;
     pdl_trigger();
     pdl_wait();
-    uint4 g[V], u[V];
+    Piece<T, E> g[V], u[V];
     auto load = [&](uint64_t at) {
         const T* pg = static_cast<const T*>(a.gate) + at * a.ld_gate;
         const T* pu = static_cast<const T*>(a.up) + at * a.ld_up;
 #pragma unroll
         for (uint32_t j = 0; j < V; j++) {
-            g[j] = load_vec<T>(pg, (t + j * G) * E, a.cols);
-            if (UP) u[j] = load_vec<T>(pu, (t + j * G) * E, a.cols);
+            load_piece<T, E>(g[j], pg, (t + j * G) * E, a.cols);
+            if (UP) load_piece<T, E>(u[j], pu, (t + j * G) * E, a.cols);
         }
     };
     if (AHEAD && row < a.rows) load(row);
@@ -202,9 +210,9 @@ __global__ void __launch_bounds__(rows_threads<WARP, V>()) glu_i8_rows_kernel(co
         float top = 0.f, unused = 0.f;
 #pragma unroll
         for (uint32_t j = 0; j < V; j++) {
-            vec_to_f32<T>(g[j], y[j]);
+            piece_to_f32<T, E>(g[j], y[j]);
             float f[E];
-            if (UP) vec_to_f32<T>(u[j], f);
+            if (UP) piece_to_f32<T, E>(u[j], f);
 #pragma unroll
             for (uint32_t i = 0; i < E; i++) {
                 y[j][i] = activate<ACT>(y[j][i]);
@@ -218,8 +226,8 @@ __global__ void __launch_bounds__(rows_threads<WARP, V>()) glu_i8_rows_kernel(co
         const RowScale s = row_scale(__uint_as_float(m));
 #pragma unroll
         for (uint32_t j = 0; j < V; j++)
-            store_quant<E>(a.q + row * a.ld_q, (t + j * G) * E, a.cols, y[j], s.inv, s, [](float v) { return v; });
-        if (t == 0) a.scale[row] = s.scale;
+            store_quant<E>(a.q + row * a.ld_q, (t + j * G) * E, a.cols, y[j], s.inv, s, s.plain(), [](float v) { return v; });
+        if (t == 0) a.scale[row] = s.scale();
     }
 }
 
@@ -236,7 +244,7 @@ struct WeightArgs {
 
 constexpr uint32_t kWSeg = 48 * 1024;      // raw bytes of a row staged at a time
 constexpr uint32_t kWRow = 96 * 1024;      // longest row that is staged whole
-constexpr uint32_t kWSlack = 192;          // behind it: the offset modulo 16, and a short last unit decoded whole
+constexpr uint32_t kWSlack = 64;           // behind it: the offset modulo 16, and words_at's read past a block
 constexpr uint32_t kWThreads = 256;
 
 
@@ -255,10 +263,14 @@ __device__ __forceinline__ void words_at(const uint8_t* p, uint32_t* w) {
         prev = nx;
     }
 }
+// Byte 0 .. 3 of a word as f32, exact: behind 0x4B it is the mantissa of 2^23 + b.
+// `off` is 2^23, or more to subtract a bias on the way.
+__device__ __forceinline__ float byte_f32(uint32_t word, int k, float off) {
+    return __fsub_rn(__uint_as_float(__byte_perm(word, 0x4B000000u, 0x7440 | k)), off);
+}
 __device__ __forceinline__ float half_at(const uint8_t* p) {
     return __half2float(*reinterpret_cast<const __half*>(p));
 }
-__device__ __forceinline__ uint32_t byte_at(const uint32_t* w, int i) { return (w[i >> 2] >> ((i & 3) * 8)) & 0xFFu; }
 
 // Elements 32 u .. 32 u + 31 of a row whose bytes (from the first block of
 // the staged segment on) are at `row`, in their own order, bit-identical to gguf.c:409-594:
@@ -266,40 +278,48 @@ __device__ __forceinline__ uint32_t byte_at(const uint32_t* w, int i) { return (
 template <uint32_t T>
 __device__ __forceinline__ void unit_weights(const uint8_t* row, uint32_t u, float* y) {
     uint32_t w[8];
+    constexpr float M = 8388608.0f;                  // 2^23
+    constexpr uint32_t nib = 0x0F0F0F0Fu;
     if constexpr (T == GGML_TYPE_Q8_0) {
         const uint8_t* b = row + (size_t)u * 34;
         const float d = half_at(b);
         words_at<8>(b + 2, w);
 #pragma unroll
-        for (int i = 0; i < 32; i++) y[i] = __fmul_rn((float)(int8_t)byte_at(w, i), d);
+        for (int i = 0; i < 32; i++) y[i] = __fmul_rn(byte_f32(w[i >> 2] ^ 0x80808080u, i & 3, M + 128.0f), d);
     } else if constexpr (T == GGML_TYPE_Q4_0) {
         const uint8_t* b = row + (size_t)u * 18;
         const float d = half_at(b);
         words_at<4>(b + 2, w);
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            y[i] = __fmul_rn((float)(int)(byte_at(w, i) & 15u) - 8.0f, d);
-            y[i + 16] = __fmul_rn((float)(int)(byte_at(w, i) >> 4) - 8.0f, d);
+            y[i] = __fmul_rn(byte_f32(w[i >> 2] & nib, i & 3, M + 8.0f), d);
+            y[i + 16] = __fmul_rn(byte_f32((w[i >> 2] >> 4) & nib, i & 3, M + 8.0f), d);
         }
     } else if constexpr (T == GGML_TYPE_Q4_1) {
+        // d q is exact (11 + 4 bits), so the fused sum rounds where gguf.c's does
         const uint8_t* b = row + (size_t)u * 20;
         const float d = half_at(b), m = half_at(b + 2);
         words_at<4>(b + 4, w);
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            y[i] = __fadd_rn(__fmul_rn((float)(byte_at(w, i) & 15u), d), m);
-            y[i + 16] = __fadd_rn(__fmul_rn((float)(byte_at(w, i) >> 4), d), m);
+            y[i] = fmaf(byte_f32(w[i >> 2] & nib, i & 3, M), d, m);
+            y[i + 16] = fmaf(byte_f32((w[i >> 2] >> 4) & nib, i & 3, M), d, m);
         }
     } else if constexpr (T == GGML_TYPE_Q5_0) {
         const uint8_t* b = row + (size_t)u * 22;
         const float d = half_at(b);
         words_at<5>(b + 2, w);
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const uint32_t lo = (byte_at(w + 1, i) & 15u) | (((w[0] >> i) & 1u) << 4);
-            const uint32_t hi = (byte_at(w + 1, i) >> 4) | (((w[0] >> (i + 16)) & 1u) << 4);
-            y[i] = __fmul_rn((float)lo - 16.0f, d);
-            y[i + 16] = __fmul_rn((float)hi - 16.0f, d);
+        for (int k = 0; k < 4; k++) {
+            // bits 4k .. 4k + 3 of the high-bit word, one to a byte, at bit 4
+            const uint32_t a = w[0] >> (4 * k), c = w[0] >> (4 * k + 16);
+            const uint32_t lo = (w[1 + k] & nib) | (((a & 1u) << 4) | ((a & 2u) << 11) | ((a & 4u) << 18) | ((a & 8u) << 25));
+            const uint32_t hi = ((w[1 + k] >> 4) & nib) | (((c & 1u) << 4) | ((c & 2u) << 11) | ((c & 4u) << 18) | ((c & 8u) << 25));
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                y[4 * k + i] = __fmul_rn(byte_f32(lo, i, M + 16.0f), d);
+                y[4 * k + i + 16] = __fmul_rn(byte_f32(hi, i, M + 16.0f), d);
+            }
         }
     } else if constexpr (T == GGML_TYPE_Q4_K || T == GGML_TYPE_Q5_K) {
         constexpr bool five = T == GGML_TYPE_Q5_K;
@@ -315,15 +335,17 @@ __device__ __forceinline__ void unit_weights(const uint8_t* row, uint32_t u, flo
             s6 = (sc[j + 4] & 15u) | ((uint32_t)(sc[j - 4] >> 6) << 4);
             m6 = (sc[j + 4] >> 4) | ((uint32_t)(sc[j] >> 6) << 4);
         }
+        // d sc and d sc q are exact (11 + 6 + 5 bits): one rounding, at the difference
         const float ds = __fmul_rn(d, (float)s6), dm = __fmul_rn(dmin, (float)m6);
         words_at<8>(b + (five ? 48 : 16) + 32 * (j >> 1), w);
         uint32_t h[8];
         if constexpr (five) words_at<8>(b + 16, h);
 #pragma unroll
-        for (int i = 0; i < 32; i++) {
-            uint32_t v = (byte_at(w, i) >> (4 * (j & 1u))) & 15u;
-            if constexpr (five) v |= ((byte_at(h, i) >> j) & 1u) << 4;
-            y[i] = __fsub_rn(__fmul_rn(ds, (float)v), dm);
+        for (int k = 0; k < 8; k++) {
+            uint32_t v = (w[k] >> (4 * (j & 1u))) & nib;
+            if constexpr (five) v |= ((h[k] >> j) & 0x01010101u) << 4;
+#pragma unroll
+            for (int i = 0; i < 4; i++) y[4 * k + i] = fmaf(ds, byte_f32(v, i, M), -dm);
         }
     } else if constexpr (T == GGML_TYPE_Q6_K) {
         const uint8_t* b = row + (size_t)(u >> 3) * 210;
@@ -335,28 +357,18 @@ __device__ __forceinline__ void unit_weights(const uint8_t* row, uint32_t u, flo
         const int8_t* sc = reinterpret_cast<const int8_t*>(b + 192 + 8 * p + 2 * c);
         const float d0 = __fmul_rn(d, (float)sc[0]), d1 = __fmul_rn(d, (float)sc[1]);
 #pragma unroll
-        for (int i = 0; i < 32; i++) {
-            const int v = (int)(((byte_at(w, i) >> (4 * (c >> 1))) & 15u) | (((byte_at(h, i) >> (2 * c)) & 3u) << 4)) - 32;
-            y[i] = __fmul_rn(i < 16 ? d0 : d1, (float)v);
+        for (int k = 0; k < 8; k++) {
+            const uint32_t v = ((w[k] >> (4 * (c >> 1))) & nib) | (((h[k] >> (2 * c)) & 0x03030303u) << 4);
+#pragma unroll
+            for (int i = 0; i < 4; i++) y[4 * k + i] = __fmul_rn(k < 4 ? d0 : d1, byte_f32(v, i, M + 32.0f));
         }
-    } else if constexpr (T == GGML_TYPE_F16) {
-        const __half* b = reinterpret_cast<const __half*>(row) + (size_t)u * 32;
-#pragma unroll
-        for (int i = 0; i < 32; i++) y[i] = __half2float(b[i]);
-    } else {
-        const float* b = reinterpret_cast<const float*>(row) + (size_t)u * 32;
-#pragma unroll
-        for (int i = 0; i < 32; i++) y[i] = b[i];
     }
 }
 
-__host__ __device__ constexpr uint32_t block_elems(uint32_t t) {
-    return t == GGML_TYPE_F32 || t == GGML_TYPE_F16 ? 1 : t >= GGML_TYPE_Q4_K ? 256 : 32;
-}
+__host__ __device__ constexpr uint32_t block_elems(uint32_t t) { return t >= GGML_TYPE_Q4_K ? 256 : 32; }
 __host__ __device__ constexpr uint32_t block_bytes(uint32_t t) {
-    return t == GGML_TYPE_F32 ? 4 : t == GGML_TYPE_F16 ? 2 : t == GGML_TYPE_Q4_0 ? 18 : t == GGML_TYPE_Q4_1 ? 20
-         : t == GGML_TYPE_Q5_0 ? 22 : t == GGML_TYPE_Q8_0 ? 34 : t == GGML_TYPE_Q4_K ? 144
-         : t == GGML_TYPE_Q5_K ? 176 : 210;
+    return t == GGML_TYPE_Q4_0 ? 18 : t == GGML_TYPE_Q4_1 ? 20 : t == GGML_TYPE_Q5_0 ? 22 : t == GGML_TYPE_Q8_0 ? 34
+         : t == GGML_TYPE_Q4_K ? 144 : t == GGML_TYPE_Q5_K ? 176 : 210;
 }
 
 // Segment `s0` (units) of a row into shared memory, at the same offset modulo
@@ -385,26 +397,24 @@ __global__ void __launch_bounds__(kWThreads) weights_i8_kernel(const WeightArgs 
     const uint64_t row = blockIdx.x;
     const uint8_t* src = a.raw + row * a.row_bytes;
     int8_t* q = a.q + row * a.ld_q;
-    const uint32_t units = (a.cols + 31) / 32;       // the last one may be short (F32, F16)
+    const uint32_t units = a.cols / 32;
     const bool whole = units <= a.seg_units;
     uint32_t m = 0;
     float unused = 0.f;
     RowScale rs = {};
     for (uint32_t pass = 0; pass < 2; pass++) {
         for (uint32_t u0 = 0; u0 < units; u0 += a.seg_units) {
-            const uint32_t nu = min(a.seg_units, units - u0), e0 = u0 * 32, ne = min(nu * 32, a.cols - e0);
+            const uint32_t nu = min(a.seg_units, units - u0), e0 = u0 * 32;
             const uint8_t* p = sm + (reinterpret_cast<uintptr_t>(src) & 15u);
             if (pass == 0 || !whole) {
                 __syncthreads();                     // the segment before has been read
-                p = stage_segment(sm, src + (uint64_t)e0 / BE * BB, ne / BE * BB);
+                p = stage_segment(sm, src + (uint64_t)e0 / BE * BB, nu * 32 / BE * BB);
             }
             for (uint32_t u = threadIdx.x; u < nu; u += kWThreads) {
                 float y[32];
                 unit_weights<T>(p, u, y);
-                const uint32_t n = min(32u, ne - u * 32);
 #pragma unroll
                 for (uint32_t i = 0; i < 32; i++) {
-                    if (i >= n) break;
                     if (pass == 0) m = max(m, abs_bits(y[i]));
                     else q[e0 + u * 32 + i] = (int8_t)quant1(y[i], rs);
                 }
@@ -415,7 +425,7 @@ __global__ void __launch_bounds__(kWThreads) weights_i8_kernel(const WeightArgs 
             rs = row_scale(__uint_as_float(m));
         }
     }
-    if (threadIdx.x == 0) a.scale[row] = rs.scale;
+    if (threadIdx.x == 0) a.scale[row] = rs.scale();
 }
 
 // The same for rows that fit: a CTA walks groups of rows (back to back in memory),
@@ -442,7 +452,7 @@ __global__ void __launch_bounds__(512, U == 1 ? 2 : 1) weights_i8_rows_kernel(co
     extern __shared__ __align__(16) uint8_t sm[];    // two buffers of `buf` bytes
     __shared__ uint32_t red[16];
     const uint32_t rows = blockDim.x / tpr, r = threadIdx.x / tpr, t = threadIdx.x - r * tpr;
-    const uint32_t units = (a.cols + 31) / 32, groups = (a.rows + rows - 1) / rows;
+    const uint32_t units = a.cols / 32, groups = (a.rows + rows - 1) / rows;
     pdl_trigger();
     pdl_wait();
     auto stage = [&](uint32_t g, uint32_t turn) {
@@ -466,20 +476,16 @@ __global__ void __launch_bounds__(512, U == 1 ? 2 : 1) weights_i8_rows_kernel(co
                 const uint32_t u = t + j * tpr;
                 if (u >= units) break;
                 unit_weights<T>(p + r * (uint32_t)a.row_bytes, u, y[j]);
-                const uint32_t left = a.cols - u * 32;
 #pragma unroll
-                for (uint32_t i = 0; i < 32; i++) {
-                    if ((T == GGML_TYPE_F32 || T == GGML_TYPE_F16) && i >= left) y[j][i] = 0.f;   // a short last unit
-                    top = max_abs(top, y[j][i]);
-                }
+                for (uint32_t i = 0; i < 32; i++) top = max_abs(top, y[j][i]);
             }
         }
         uint32_t m = __reduce_max_sync(0xffffffffu, abs_bits(top));
         if ((threadIdx.x & 31u) == 0) red[threadIdx.x >> 5] = m;
         __syncthreads();                             // (and every thread has read this buffer)
         if (row >= a.rows) continue;
-        m = 0;
-        for (uint32_t i = 0; i < tpr / 32; i++) m = max(m, red[r * (tpr / 32) + i]);
+        const uint32_t nw = tpr / 32, lane = threadIdx.x & 31u;
+        m = __reduce_max_sync(0xffffffffu, lane < nw ? red[r * nw + lane] : 0u);
         const RowScale rs = row_scale(__uint_as_float(m));
         int8_t* q = a.q + row * a.ld_q;
         const bool odd = t & 1u;
@@ -487,7 +493,7 @@ __global__ void __launch_bounds__(512, U == 1 ? 2 : 1) weights_i8_rows_kernel(co
         for (uint32_t j = 0; j < U; j++) {
             const uint32_t u = t + j * tpr;
             uint32_t w[8];
-            if (!rs.zero && !rs.tiny) {
+            if (rs.plain()) {
 #pragma unroll
                 for (uint32_t i = 0; i < 8; i++)
                     w[i] = low_bytes(fmaf(y[j][4 * i], rs.inv, kRound), fmaf(y[j][4 * i + 1], rs.inv, kRound),
@@ -511,24 +517,18 @@ __global__ void __launch_bounds__(512, U == 1 ? 2 : 1) weights_i8_rows_kernel(co
                 s1[i] = odd ? got : w[i];
                 s2[i] = odd ? w[4 + i] : got;
             }
-            const uint32_t e1 = (u & ~1u) * 32 + (odd ? 16 : 0), e2 = e1 + 32;
-            if (e1 + 16 <= a.cols) *reinterpret_cast<uint4*>(q + e1) = make_uint4(s1[0], s1[1], s1[2], s1[3]);
-            else
-                for (uint32_t i = 0; i < 16; i++)
-                    if (e1 + i < a.cols) q[e1 + i] = (int8_t)(s1[i >> 2] >> (8 * (i & 3u)));
-            if (e2 + 16 <= a.cols) *reinterpret_cast<uint4*>(q + e2) = make_uint4(s2[0], s2[1], s2[2], s2[3]);
-            else
-                for (uint32_t i = 0; i < 16; i++)
-                    if (e2 + i < a.cols) q[e2 + i] = (int8_t)(s2[i >> 2] >> (8 * (i & 3u)));
+            int8_t* o = q + (u & ~1u) * 32 + (odd ? 16 : 0);
+            if ((u & ~1u) < units) *reinterpret_cast<uint4*>(o) = make_uint4(s1[0], s1[1], s1[2], s1[3]);
+            if ((u | 1u) < units) *reinterpret_cast<uint4*>(o + 32) = make_uint4(s2[0], s2[1], s2[2], s2[3]);
         }
-        if (t == 0) a.scale[row] = rs.scale;
+        if (t == 0) a.scale[row] = rs.scale();
     }
 }
 
 template <uint32_t T>
 bool launch_weights(const WeightArgs& a, cudaStream_t st) {
     // rows of up to 1024 units whose int8 rows start on 16 bytes
-    const uint32_t units = (a.cols + 31) / 32, U = units <= 512 ? 1 : 2, tpr = (units + 32 * U - 1) / (32 * U) * 32;
+    const uint32_t units = a.cols / 32, U = units <= 512 ? 1 : 2, tpr = (units + 32 * U - 1) / (32 * U) * 32;
     if (tpr <= 512 && i8_aligned(a.q, 16) && a.ld_q % 16 == 0 && a.row_bytes <= kWRow) {
         uint32_t rows = tpr < 256 ? 256 / tpr : 1;   // about 256 threads a CTA
         while (rows > 1 && rows * a.row_bytes > kWRow / 4) rows--;
@@ -613,59 +613,72 @@ struct RowShape {
     uint32_t threads, per;
 };
 
-template <typename T, bool RESID, bool WARP, uint32_t V>
+template <typename T, bool RESID, uint32_t E, bool WARP, uint32_t V>
 bool launch_norm_rows(const NormArgs& a, const RowShape& r, cudaStream_t st) {
     static std::atomic<int> occupancy[33];
-    const uint32_t grid = walkers(occupancy, norm_i8_rows_kernel<T, RESID, WARP, V>, r.threads, a.rows, r.per);
-    return LM_CUDA(launch_k(norm_i8_rows_kernel<T, RESID, WARP, V>, dim3(grid), dim3(r.threads), 0, st, a));
+    const uint32_t grid = walkers(occupancy, norm_i8_rows_kernel<T, RESID, WARP, E, V>, r.threads, a.rows, r.per);
+    return LM_CUDA(launch_k(norm_i8_rows_kernel<T, RESID, WARP, E, V>, dim3(grid), dim3(r.threads), 0, st, a));
 }
-template <typename T, uint32_t ACT, bool UP, bool WARP, uint32_t V>
+template <typename T, uint32_t ACT, bool UP, uint32_t E, bool WARP, uint32_t V>
 bool launch_glu_rows(const GluArgs& a, const RowShape& r, cudaStream_t st) {
     static std::atomic<int> occupancy[33];
-    const uint32_t grid = walkers(occupancy, glu_i8_rows_kernel<T, ACT, UP, WARP, V>, r.threads, a.rows, r.per);
-    return LM_CUDA(launch_k(glu_i8_rows_kernel<T, ACT, UP, WARP, V>, dim3(grid), dim3(r.threads), 0, st, a));
+    const uint32_t grid = walkers(occupancy, glu_i8_rows_kernel<T, ACT, UP, WARP, E, V>, r.threads, a.rows, r.per);
+    return LM_CUDA(launch_k(glu_i8_rows_kernel<T, ACT, UP, WARP, E, V>, dim3(grid), dim3(r.threads), 0, st, a));
 }
 
 // Calls LAUNCH for the shape that fits rows of `cols` elements; falls through
 // when no shape does.
-#define LM_I8_ROWS(LAUNCH, ...)                                                             \
+#define LM_I8_VEC_ROWS(LAUNCH, T, ...)                                                      \
     do {                                                                                    \
-        const uint32_t nv = (a.cols + vec_elems<T>() - 1) / vec_elems<T>();                 \
-        int tv = getenv("I8_V") ? atoi(getenv("I8_V")) : 0;                          \
-        const uint32_t V = tv ? tv : rows_vectors(a.rows, nv);                                   \
+        constexpr uint32_t E = vec_elems<T>();                                              \
+        const uint32_t nv = (a.cols + E - 1) / E;                                           \
+        int tv = getenv("I8_V") ? atoi(getenv("I8_V")) : 0;                                 \
+        const uint32_t V = tv ? tv : rows_vectors(a.rows, nv);                              \
         if (V % 10 == 0) break;                                                             \
         const RowShape w = {32 * kWarpRows, kWarpRows}, r = {((nv + V % 10 - 1) / (V % 10) + 31) / 32 * 32, 1}; \
-        if (V > 10 ? nv > 32 * (V - 10) : r.threads > (V > 1 ? 512u : 1024u)) break;       \
+        if (V > 10 ? nv > 32 * (V - 10) : r.threads > (V * E > 8 ? 512u : 1024u)) break;    \
         switch (V) {                                                                        \
-        case 11: return LAUNCH<__VA_ARGS__, true, 1>(a, w, st);                             \
-        case 12: return LAUNCH<__VA_ARGS__, true, 2>(a, w, st);                             \
-        case 14: return LAUNCH<__VA_ARGS__, true, 4>(a, w, st);                             \
-        case 1: return LAUNCH<__VA_ARGS__, false, 1>(a, r, st);                             \
-        case 2: return LAUNCH<__VA_ARGS__, false, 2>(a, r, st);                             \
-        case 3: return LAUNCH<__VA_ARGS__, false, 3>(a, r, st);                             \
-        case 4: return LAUNCH<__VA_ARGS__, false, 4>(a, r, st);                             \
-        case 8: return LAUNCH<__VA_ARGS__, false, 8>(a, r, st);                             \
+        case 11: return LAUNCH<T, __VA_ARGS__, E, true, 1>(a, w, st);                       \
+        case 12: return LAUNCH<T, __VA_ARGS__, E, true, 2>(a, w, st);                       \
+        case 1: return LAUNCH<T, __VA_ARGS__, E, false, 1>(a, r, st);                       \
+        case 2: return LAUNCH<T, __VA_ARGS__, E, false, 2>(a, r, st);                       \
+        case 3: return LAUNCH<T, __VA_ARGS__, E, false, 3>(a, r, st);                       \
+        case 4: return LAUNCH<T, __VA_ARGS__, E, false, 4>(a, r, st);                       \
+        case 6: return LAUNCH<T, __VA_ARGS__, E, false, 6>(a, r, st);                       \
+        case 8: return LAUNCH<T, __VA_ARGS__, E, false, 8>(a, r, st);                       \
         }                                                                                   \
+    } while (0)
+// The same one element at a time.
+#define LM_I8_ODD_ROWS(LAUNCH, T, ...)                                                      \
+    do {                                                                                    \
+        const uint32_t n = a.cols;                                                          \
+        const RowShape w = {32 * kWarpRows, kWarpRows}, r = {((n + 7) / 8 + 31) / 32 * 32, 1}, \
+                       s = {((n + 31) / 32 + 31) / 32 * 32, 1};                             \
+        if (a.rows >= 1024 && n <= 256) return LAUNCH<T, __VA_ARGS__, 1, true, 8>(a, w, st); \
+        if (n <= 4096) return LAUNCH<T, __VA_ARGS__, 1, false, 8>(a, r, st);                \
+        if (n <= 16384) return LAUNCH<T, __VA_ARGS__, 1, false, 32>(a, s, st);              \
     } while (0)
 
 uint32_t rows_vectors(uint32_t rows, uint32_t nv) {
     if (rows >= 1024 && nv <= 32) return 11;
     if (rows >= 1024 && nv <= 64) return 12;
-    if (rows >= 1024 && nv <= 128) return 14;
     if (nv <= 128) return 1;
     if (nv <= 1024) return 2;
     if (nv <= 2048) return 4;
     return nv <= 4096 ? 8 : 0;
 }
 
-template <typename T, uint32_t ACT>
-bool launch_glu_act(const GluArgs& a, cudaStream_t st) {
-    if (vec_rows<T>(a.gate, a.ld_gate) && vec_rows<T>(a.up, a.ld_up) && vec_q<T>(a.q, a.ld_q)) {
-        if (a.up) LM_I8_ROWS(launch_glu_rows, T, ACT, true);
-        else LM_I8_ROWS(launch_glu_rows, T, ACT, false);
-    }
+template <typename T, uint32_t ACT, bool UP>
+bool launch_glu_up(const GluArgs& a, cudaStream_t st) {
+    if (vec_rows<T>(a.gate, a.ld_gate) && vec_rows<T>(a.up, a.ld_up) && vec_q<T>(a.q, a.ld_q))
+        LM_I8_VEC_ROWS(launch_glu_rows, T, ACT, UP);
+    LM_I8_ODD_ROWS(launch_glu_rows, T, ACT, UP);
     glu_i8_kernel<T, ACT><<<a.rows, 256, 0, st>>>(a);
     return LM_CUDA(cudaGetLastError());
+}
+template <typename T, uint32_t ACT>
+bool launch_glu_act(const GluArgs& a, cudaStream_t st) {
+    return a.up ? launch_glu_up<T, ACT, true>(a, st) : launch_glu_up<T, ACT, false>(a, st);
 }
 template <typename T>
 bool launch_glu(const GluArgs& a, cudaStream_t st) {
@@ -673,15 +686,17 @@ bool launch_glu(const GluArgs& a, cudaStream_t st) {
     if (a.act == ACT_GELU) return launch_glu_act<T, ACT_GELU>(a, st);
     return launch_glu_act<T, LLAMINI_ACT_NONE>(a, st);
 }
-template <typename T>
+template <typename T, bool RESID>
 bool launch_norm(const NormArgs& a, cudaStream_t st) {
-    if (vec_rows<T>(a.x, a.ld_x) && vec_rows<T>(a.resid, a.ld_resid) && vec_rows<T>(a.sum, a.ld_sum) &&
-        i8_aligned(a.w, 16) && vec_q<T>(a.q, a.ld_q)) {
-        if (a.resid) LM_I8_ROWS(launch_norm_rows, T, true);
-        else LM_I8_ROWS(launch_norm_rows, T, false);
-    }
+    if (vec_rows<T>(a.x, a.ld_x) && vec_rows<T>(a.resid, a.ld_resid) && vec_rows<T>(a.sum, a.ld_sum) && vec_q<T>(a.q, a.ld_q))
+        LM_I8_VEC_ROWS(launch_norm_rows, T, RESID);
+    LM_I8_ODD_ROWS(launch_norm_rows, T, RESID);
     norm_i8_kernel<T><<<a.rows, 256, 0, st>>>(a);
     return LM_CUDA(cudaGetLastError());
+}
+template <typename T>
+bool launch_norm(const NormArgs& a, cudaStream_t st) {
+    return a.resid ? launch_norm<T, true>(a, st) : launch_norm<T, false>(a, st);
 }
 
 }  // namespace
@@ -710,14 +725,17 @@ extern "C" int llamini_weights_i8_device(u32 type, const void* d_blocks, u32 row
     a.row_bytes = type_bytes(type, cols);
     a.ld_q = ld_q;
     a.rows = rows; a.cols = cols; a.type = type;
-    // whole blocks, and whole 32-element units, to a segment
-    const uint32_t per = ti.block_elems >= 32 ? ti.block_elems : 32;
-    a.seg_units = kWSeg / (per / ti.block_elems * ti.block_bytes) * (per / 32);
+    a.seg_units = kWSeg / ti.block_bytes * (ti.block_elems / 32);    // whole blocks to a segment
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     bool ok = false;
+    GluArgs g = {};                                  // plain rows: the rounding of the gated activation without one
+    g.gate = d_blocks;
+    g.q = a.q; g.scale = a.scale;
+    g.ld_gate = cols; g.ld_q = ld_q;
+    g.rows = rows; g.cols = cols; g.act = LLAMINI_ACT_NONE;
     switch (type) {
-    case GGML_TYPE_F32: ok = launch_weights<GGML_TYPE_F32>(a, st); break;
-    case GGML_TYPE_F16: ok = launch_weights<GGML_TYPE_F16>(a, st); break;
+    case GGML_TYPE_F32: ok = launch_glu<float>(g, st); break;
+    case GGML_TYPE_F16: ok = launch_glu<__half>(g, st); break;
     case GGML_TYPE_Q4_0: ok = launch_weights<GGML_TYPE_Q4_0>(a, st); break;
     case GGML_TYPE_Q4_1: ok = launch_weights<GGML_TYPE_Q4_1>(a, st); break;
     case GGML_TYPE_Q5_0: ok = launch_weights<GGML_TYPE_Q5_0>(a, st); break;
