@@ -10,7 +10,7 @@
 // fused multiply-add, exact and the same everywhere.) A row of zeros has scale 0.
 // A row that holds a NaN or an infinity has scale NaN and q = 0: every value it
 // stands for is NaN, so the fault stays visible. Where 127 / max|y| would
-// overflow (max|y| below 1.5e-36) q is y / scale instead, within -127 to 127.
+// overflow (max|y| below 1.5e-36) y and max|y| are multiplied by 2^100 first.
 #pragma once
 
 #include "internal.h"
@@ -102,27 +102,24 @@ constexpr float kRound = 12582912.0f;
 // How the elements of a row with this largest magnitude become integers, and
 // the row's scale (a division that only one thread of a row needs).
 struct RowScale {
-    float amax, inv;
-    bool bad, tiny;            // NaN or infinity in the row; 127 / amax overflows (or the row is zero)
-    __device__ __forceinline__ float scale() const { return bad ? NAN : __fdiv_rn(amax, 127.0f); }
-    __device__ __forceinline__ bool plain() const { return !bad && !tiny; }
+    float amax, inv, up;       // 127 / (amax up); up = 1, or 2^100 for tiny rows
+    bool plain;                // finite and not tiny: q = y inv
+    __device__ __forceinline__ float scale() const { return amax < INFINITY ? __fdiv_rn(amax, 127.0f) : NAN; }
+    // what a row that is not plain multiplies by inv: nothing is left of one that
+    // is not finite or whose scale rounds to zero
+    __device__ __forceinline__ float odd(float y) const { return scale() > 0.0f ? y * up : 0.0f; }
 };
 __device__ __forceinline__ RowScale row_scale(float amax) {
     RowScale r;
     r.amax = amax;
-    r.bad = !(amax < INFINITY);
-    r.tiny = amax < 1.5e-36f;
-    r.inv = __fdiv_rn(127.0f, amax);
+    r.plain = amax >= 1.5e-36f && amax < INFINITY;
+    r.up = amax < 1.5e-36f ? 0x1p100f : 1.0f;
+    r.inv = r.plain || amax > 0.0f ? __fdiv_rn(127.0f, amax * r.up) : 0.0f;
+    if (!(amax < INFINITY)) r.inv = 0.0f;
     return r;
 }
-// One element of a row; out of line where the row is not plain.
-inline __device__ __noinline__ int quant_odd(float y, const RowScale r) {
-    const float s = r.scale();
-    if (r.bad || s == 0.0f) return 0;
-    return max(-127, min(127, __float2int_rn(__fdiv_rn(y, s))));
-}
 __device__ __forceinline__ int quant1(float y, const RowScale& r) {
-    return r.plain() ? (int)(int8_t)__float_as_uint(fmaf(y, r.inv, kRound)) : quant_odd(y, r);
+    return (int)(int8_t)__float_as_uint(fmaf(r.plain ? y : r.odd(y), r.inv, kRound));
 }
 
 // Block-wide maximum of unsigned integers and sum of floats; every thread gets
@@ -241,27 +238,16 @@ __device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d
 }
 
 // E values of a row, times f (127 / max, or what maps onto it), to int8 at q + at.
-// Rows that are not plain go by y(value), what the row's scale is of.
-template <uint32_t E, typename Y>
-__device__ __forceinline__ void store_quant(int8_t* q, uint32_t at, uint32_t cols, const float* v, float f,
-                                            const RowScale& r, bool plain, Y y) {
+template <uint32_t E>
+__device__ __forceinline__ void store_quant(int8_t* q, uint32_t at, uint32_t cols, const float* v, float f) {
     if constexpr (E == 1) {
-        if (at < cols) q[at] = plain ? (int8_t)__float_as_uint(fmaf(v[0], f, kRound)) : (int8_t)quant_odd(y(v[0]), r);
+        if (at < cols) q[at] = (int8_t)__float_as_uint(fmaf(v[0], f, kRound));
     } else {
         uint32_t w[E / 4];
-        if (plain) {
 #pragma unroll
-            for (uint32_t i = 0; i < E / 4; i++)
-                w[i] = low_bytes(fmaf(v[4 * i], f, kRound), fmaf(v[4 * i + 1], f, kRound), fmaf(v[4 * i + 2], f, kRound),
-                                 fmaf(v[4 * i + 3], f, kRound));
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < E / 4; i++) {
-                w[i] = 0;
-#pragma unroll
-                for (uint32_t j = 0; j < 4; j++) w[i] |= ((uint32_t)quant_odd(y(v[4 * i + j]), r) & 0xFFu) << (8 * j);
-            }
-        }
+        for (uint32_t i = 0; i < E / 4; i++)
+            w[i] = low_bytes(fmaf(v[4 * i], f, kRound), fmaf(v[4 * i + 1], f, kRound), fmaf(v[4 * i + 2], f, kRound),
+                             fmaf(v[4 * i + 3], f, kRound));
         if (at + E <= cols) {
             if constexpr (E == 8) *reinterpret_cast<uint2*>(q + at) = make_uint2(w[0], w[1]);
             else *reinterpret_cast<uint32_t*>(q + at) = w[0];

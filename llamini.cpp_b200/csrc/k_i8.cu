@@ -15,8 +15,12 @@ namespace lm {
 namespace {
 
 constexpr uint32_t kWarpRows = 8;          // rows at a time of a CTA whose warps have one each
-// The most threads of a CTA that keeps up to N elements a thread in registers.
-template <bool WARP, uint32_t N> constexpr uint32_t rows_threads() { return WARP ? 32 * kWarpRows : N > 8 ? 512 : 1024; }
+// The most threads of a CTA that keeps up to V pieces of E elements a thread in
+// registers, and whether the next row's pieces fit there too.
+template <bool WARP, uint32_t E, uint32_t V> constexpr uint32_t rows_threads() {
+    return WARP ? 32 * kWarpRows : V * E <= 8 || E == 1 ? 1024 : 512;
+}
+template <uint32_t E, uint32_t V> constexpr bool rows_ahead() { return V * E <= (E == 1 ? 8 : 32); }
 
 // ---------------------------------------------------------------- norm
 
@@ -65,9 +69,9 @@ __global__ void __launch_bounds__(256) norm_i8_kernel(const NormArgs a) {
 // h w of every element is kept from the first pass to the second. CTAs walk the
 // rows with w in registers and the next row's loads in flight.
 template <typename T, bool RESID, bool WARP, uint32_t E, uint32_t V>
-__global__ void __launch_bounds__(rows_threads<WARP, V * E>()) norm_i8_rows_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(rows_threads<WARP, E, V>()) norm_i8_rows_kernel(const NormArgs a) {
     constexpr uint32_t R = WARP ? kWarpRows : 1;     // rows of a CTA at a time
-    constexpr bool AHEAD = V * E <= 32;              // the next row's vectors fit the registers too
+    constexpr bool AHEAD = rows_ahead<E, V>();
     __shared__ uint32_t red[WARP ? 1 : 128];
     const uint32_t G = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31u : threadIdx.x;
     uint64_t row = (uint64_t)blockIdx.x * R + (WARP ? threadIdx.x >> 5 : 0);
@@ -120,11 +124,16 @@ __global__ void __launch_bounds__(rows_threads<WARP, V * E>()) norm_i8_rows_kern
         row_max_sum<WARP>(m, ss, red, turn);
         const float rstd = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
         const RowScale s = row_scale(__uint_as_float(m) * rstd);
-        const float f = rstd * s.inv;
-        const bool plain = s.plain() && f < INFINITY;
+        float f = rstd * s.inv;
+        if (!(s.plain && f < INFINITY)) {            // in two steps
 #pragma unroll
-        for (uint32_t j = 0; j < V; j++)
-            store_quant<E>(a.q + row * a.ld_q, (t + j * G) * E, a.cols, hw[j], f, s, plain, [&](float v) { return v * rstd; });
+            for (uint32_t j = 0; j < V; j++)
+#pragma unroll
+                for (uint32_t i = 0; i < E; i++) hw[j][i] = s.odd(hw[j][i] * rstd);
+            f = s.inv;
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < V; j++) store_quant<E>(a.q + row * a.ld_q, (t + j * G) * E, a.cols, hw[j], f);
         if (t == 0) a.scale[row] = s.scale();
     }
 }
@@ -184,9 +193,9 @@ __global__ void __launch_bounds__(256) glu_i8_kernel(const GluArgs a) {
 // The same with a row's values in the registers of G threads, read and
 // activated once; the next row's loads are in flight meanwhile.
 template <typename T, uint32_t ACT, bool UP, bool WARP, uint32_t E, uint32_t V>
-__global__ void __launch_bounds__(rows_threads<WARP, V * E>()) glu_i8_rows_kernel(const GluArgs a) {
+__global__ void __launch_bounds__(rows_threads<WARP, E, V>()) glu_i8_rows_kernel(const GluArgs a) {
     constexpr uint32_t R = WARP ? kWarpRows : 1;
-    constexpr bool AHEAD = V * E <= 32;
+    constexpr bool AHEAD = rows_ahead<E, V>();
     __shared__ uint32_t red[WARP ? 1 : 128];
     const uint32_t G = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31u : threadIdx.x;
     uint64_t row = (uint64_t)blockIdx.x * R + (WARP ? threadIdx.x >> 5 : 0);
@@ -224,9 +233,14 @@ __global__ void __launch_bounds__(rows_threads<WARP, V * E>()) glu_i8_rows_kerne
         uint32_t m = abs_bits(top);
         row_max_sum<WARP>(m, unused, red, turn);
         const RowScale s = row_scale(__uint_as_float(m));
+        if (!s.plain) {
 #pragma unroll
-        for (uint32_t j = 0; j < V; j++)
-            store_quant<E>(a.q + row * a.ld_q, (t + j * G) * E, a.cols, y[j], s.inv, s, s.plain(), [](float v) { return v; });
+            for (uint32_t j = 0; j < V; j++)
+#pragma unroll
+                for (uint32_t i = 0; i < E; i++) y[j][i] = s.odd(y[j][i]);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < V; j++) store_quant<E>(a.q + row * a.ld_q, (t + j * G) * E, a.cols, y[j], s.inv);
         if (t == 0) a.scale[row] = s.scale();
     }
 }
@@ -492,20 +506,15 @@ __global__ void __launch_bounds__(512, U == 1 ? 2 : 1) weights_i8_rows_kernel(co
 #pragma unroll
         for (uint32_t j = 0; j < U; j++) {
             const uint32_t u = t + j * tpr;
-            uint32_t w[8];
-            if (rs.plain()) {
+            if (!rs.plain) {
 #pragma unroll
-                for (uint32_t i = 0; i < 8; i++)
-                    w[i] = low_bytes(fmaf(y[j][4 * i], rs.inv, kRound), fmaf(y[j][4 * i + 1], rs.inv, kRound),
-                                     fmaf(y[j][4 * i + 2], rs.inv, kRound), fmaf(y[j][4 * i + 3], rs.inv, kRound));
-            } else {
-#pragma unroll
-                for (uint32_t i = 0; i < 8; i++) {
-                    w[i] = 0;
-#pragma unroll
-                    for (uint32_t k = 0; k < 4; k++) w[i] |= ((uint32_t)quant1(y[j][4 * i + k], rs) & 0xFFu) << (8 * k);
-                }
+                for (uint32_t i = 0; i < 32; i++) y[j][i] = rs.odd(y[j][i]);
             }
+            uint32_t w[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++)
+                w[i] = low_bytes(fmaf(y[j][4 * i], rs.inv, kRound), fmaf(y[j][4 * i + 1], rs.inv, kRound),
+                                 fmaf(y[j][4 * i + 2], rs.inv, kRound), fmaf(y[j][4 * i + 3], rs.inv, kRound));
             // 32 bytes a unit: the even lane stores the first 16 of its own unit, the
             // odd one the second 16 of that, then the same for the odd lane's unit,
             // so that a store covers whole 32-byte sectors (lanes without a unit take part)
@@ -653,10 +662,10 @@ bool launch_glu_rows(const GluArgs& a, const RowShape& r, cudaStream_t st) {
     do {                                                                                    \
         const uint32_t n = a.cols;                                                          \
         const RowShape w = {32 * kWarpRows, kWarpRows}, r = {((n + 7) / 8 + 31) / 32 * 32, 1}, \
-                       s = {((n + 31) / 32 + 31) / 32 * 32, 1};                             \
+                       s = {((n + 15) / 16 + 31) / 32 * 32, 1};                             \
         if (a.rows >= 1024 && n <= 256) return LAUNCH<T, __VA_ARGS__, 1, true, 8>(a, w, st); \
-        if (n <= 4096) return LAUNCH<T, __VA_ARGS__, 1, false, 8>(a, r, st);                \
-        if (n <= 16384) return LAUNCH<T, __VA_ARGS__, 1, false, 32>(a, s, st);              \
+        if (n <= 8192) return LAUNCH<T, __VA_ARGS__, 1, false, 8>(a, r, st);                \
+        if (n <= 16384) return LAUNCH<T, __VA_ARGS__, 1, false, 16>(a, s, st);              \
     } while (0)
 
 uint32_t rows_vectors(uint32_t rows, uint32_t nv) {
