@@ -9,7 +9,6 @@
 #include "pdl.cuh"
 
 #include <atomic>
-#include <cstdlib>
 
 namespace lm {
 namespace {
@@ -41,7 +40,7 @@ struct NormArgs {
 // element before the same thread overwrites it, in the second pass, so the sum
 // may be stored over x or the residual.
 template <typename T>
-__global__ void __launch_bounds__(256) norm_i8_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(512) norm_i8_kernel(const NormArgs a) {
     __shared__ uint32_t red[64];
     const uint64_t row = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
@@ -162,19 +161,18 @@ __device__ __forceinline__ float sigmoid_of(float minus_z_log2e) {
     asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(1.0f + e));
     return r;
 }
-template <uint32_t ACT>
-__device__ __forceinline__ float activate(float x) {
+__device__ __forceinline__ float activate(float x, uint32_t act) {
     constexpr float log2e = 1.4426950408889634f;
-    if (ACT == ACT_SILU) return x * sigmoid_of(x * -log2e);
-    if (ACT == ACT_GELU) {
+    if (act == ACT_SILU) return x * sigmoid_of(x * -log2e);
+    if (act == ACT_GELU) {
         constexpr float k = -2.0f * 0.79788456080286535587989211986876f * log2e;
         return x * sigmoid_of(x * fmaf(0.044715f * k, x * x, k));
     }
     return x;
 }
 
-template <typename T, uint32_t ACT>
-__global__ void __launch_bounds__(256) glu_i8_kernel(const GluArgs a) {
+template <typename T>
+__global__ void __launch_bounds__(512) glu_i8_kernel(const GluArgs a) {
     __shared__ uint32_t red[64];
     const uint64_t row = blockIdx.x;
     const T* g = static_cast<const T*>(a.gate) + row * a.ld_gate;
@@ -182,17 +180,17 @@ __global__ void __launch_bounds__(256) glu_i8_kernel(const GluArgs a) {
     uint32_t m = 0;
     float unused = 0.f;
     for (uint32_t i = threadIdx.x; i < a.cols; i += blockDim.x)
-        m = max(m, abs_bits(activate<ACT>(to_f32(g[i])) * (u ? to_f32(u[i]) : 1.f)));
+        m = max(m, abs_bits(activate(to_f32(g[i]), a.act) * (u ? to_f32(u[i]) : 1.f)));
     block_max_sum(m, unused, red);
     const RowScale s = row_scale(__uint_as_float(m));
     for (uint32_t i = threadIdx.x; i < a.cols; i += blockDim.x)
-        a.q[row * a.ld_q + i] = (int8_t)quant1(activate<ACT>(to_f32(g[i])) * (u ? to_f32(u[i]) : 1.f), s);
+        a.q[row * a.ld_q + i] = (int8_t)quant1(activate(to_f32(g[i]), a.act) * (u ? to_f32(u[i]) : 1.f), s);
     if (threadIdx.x == 0) a.scale[row] = s.scale();
 }
 
 // The same with a row's values in the registers of G threads, read and
 // activated once; the next row's loads are in flight meanwhile.
-template <typename T, uint32_t ACT, bool UP, bool WARP, uint32_t E, uint32_t V>
+template <typename T, bool UP, bool WARP, uint32_t E, uint32_t V>
 __global__ void __launch_bounds__(rows_threads<WARP, E, V>()) glu_i8_rows_kernel(const GluArgs a) {
     constexpr uint32_t R = WARP ? kWarpRows : 1;
     constexpr bool AHEAD = rows_ahead<E, V>();
@@ -220,11 +218,17 @@ __global__ void __launch_bounds__(rows_threads<WARP, E, V>()) glu_i8_rows_kernel
 #pragma unroll
         for (uint32_t j = 0; j < V; j++) {
             piece_to_f32<T, E>(g[j], y[j]);
+            if (a.act == ACT_SILU) {                 // (one branch a piece, the same for all)
+#pragma unroll
+                for (uint32_t i = 0; i < E; i++) y[j][i] = activate(y[j][i], ACT_SILU);
+            } else if (a.act == ACT_GELU) {
+#pragma unroll
+                for (uint32_t i = 0; i < E; i++) y[j][i] = activate(y[j][i], ACT_GELU);
+            }
             float f[E];
             if (UP) piece_to_f32<T, E>(u[j], f);
 #pragma unroll
             for (uint32_t i = 0; i < E; i++) {
-                y[j][i] = activate<ACT>(y[j][i]);
                 if (UP) y[j][i] *= f[i];
                 top = max_abs(top, y[j][i]);
             }
@@ -628,25 +632,39 @@ bool launch_norm_rows(const NormArgs& a, const RowShape& r, cudaStream_t st) {
     const uint32_t grid = walkers(occupancy, norm_i8_rows_kernel<T, RESID, WARP, E, V>, r.threads, a.rows, r.per);
     return LM_CUDA(launch_k(norm_i8_rows_kernel<T, RESID, WARP, E, V>, dim3(grid), dim3(r.threads), 0, st, a));
 }
-template <typename T, uint32_t ACT, bool UP, uint32_t E, bool WARP, uint32_t V>
+template <typename T, bool UP, uint32_t E, bool WARP, uint32_t V>
 bool launch_glu_rows(const GluArgs& a, const RowShape& r, cudaStream_t st) {
     static std::atomic<int> occupancy[33];
-    const uint32_t grid = walkers(occupancy, glu_i8_rows_kernel<T, ACT, UP, WARP, E, V>, r.threads, a.rows, r.per);
-    return LM_CUDA(launch_k(glu_i8_rows_kernel<T, ACT, UP, WARP, E, V>, dim3(grid), dim3(r.threads), 0, st, a));
+    const uint32_t grid = walkers(occupancy, glu_i8_rows_kernel<T, UP, WARP, E, V>, r.threads, a.rows, r.per);
+    return LM_CUDA(launch_k(glu_i8_rows_kernel<T, UP, WARP, E, V>, dim3(grid), dim3(r.threads), 0, st, a));
+}
+
+// Vectors a thread for rows of nv 16-byte vectors (0: none fits; 10 + V: V a lane,
+// a warp a row). Few and short rows want one vector a thread, for the shortest
+// path through a row; long ones enough threads for two CTAs an SM and no idle lanes
+// in the last round. us of bf16 norm with residual at V = 1, 2, 4: 4096 x 2048
+// 11.8, 12.6, 13.1; 4096 x 4096 21.7, 22.6, 21.1. bf16 SiLU at V = 2, 3, 4: 4096 x
+// 4864 19.4, 22.7, 20.8; 4096 x 11008 (3, 4, 6) 47.0, 51.2, 46.9; f32 (6, 8) 63.2, 68.5.
+// Many short rows, a warp each: 20000 x 128 bf16 norm 8.2 against 10.1 us.
+uint32_t rows_vectors(bool norm, uint32_t rows, uint32_t nv) {
+    if (rows >= 1024 && nv <= 32) return 11;
+    if (rows >= 1024 && nv <= 64) return 12;
+    if (nv <= 256) return 1;
+    if (nv <= 1024) return norm && rows >= 1024 && nv >= 512 ? 4 : 2;
+    if (nv <= 1536) return 3;
+    if (nv <= 2048) return 4;
+    return nv <= 3072 ? 6 : nv <= 4096 ? 8 : 0;
 }
 
 // Calls LAUNCH for the shape that fits rows of `cols` elements; falls through
 // when no shape does.
-#define LM_I8_VEC_ROWS(LAUNCH, T, ...)                                                      \
+#define LM_I8_VEC_ROWS(NORM, LAUNCH, T, ...)                                                \
     do {                                                                                    \
         constexpr uint32_t E = vec_elems<T>();                                              \
-        const uint32_t nv = (a.cols + E - 1) / E;                                           \
-        int tv = getenv("I8_V") ? atoi(getenv("I8_V")) : 0;                                 \
-        const uint32_t V = tv ? tv : rows_vectors(a.rows, nv);                              \
-        if (V % 10 == 0) break;                                                             \
-        const RowShape w = {32 * kWarpRows, kWarpRows}, r = {((nv + V % 10 - 1) / (V % 10) + 31) / 32 * 32, 1}; \
-        if (V > 10 ? nv > 32 * (V - 10) : r.threads > (V * E > 8 ? 512u : 1024u)) break;    \
-        switch (V) {                                                                        \
+        const uint32_t nv = (a.cols + E - 1) / E, v = rows_vectors(NORM, a.rows, nv);       \
+        if (v == 0) break;                                                                  \
+        const RowShape w = {32 * kWarpRows, kWarpRows}, r = {((nv + v - 1) / v + 31) / 32 * 32, 1}; \
+        switch (v) {                                                                        \
         case 11: return LAUNCH<T, __VA_ARGS__, E, true, 1>(a, w, st);                       \
         case 12: return LAUNCH<T, __VA_ARGS__, E, true, 2>(a, w, st);                       \
         case 1: return LAUNCH<T, __VA_ARGS__, E, false, 1>(a, r, st);                       \
@@ -657,7 +675,8 @@ bool launch_glu_rows(const GluArgs& a, const RowShape& r, cudaStream_t st) {
         case 8: return LAUNCH<T, __VA_ARGS__, E, false, 8>(a, r, st);                       \
         }                                                                                   \
     } while (0)
-// The same one element at a time.
+// The same one element at a time, where a pitch or base is not whole 16-byte
+// vectors (4096 x 4097 bf16 norm: 62 us; 4096 x 4096 from vectors 21).
 #define LM_I8_ODD_ROWS(LAUNCH, T, ...)                                                      \
     do {                                                                                    \
         const uint32_t n = a.cols;                                                          \
@@ -668,39 +687,25 @@ bool launch_glu_rows(const GluArgs& a, const RowShape& r, cudaStream_t st) {
         if (n <= 16384) return LAUNCH<T, __VA_ARGS__, 1, false, 16>(a, s, st);              \
     } while (0)
 
-uint32_t rows_vectors(uint32_t rows, uint32_t nv) {
-    if (rows >= 1024 && nv <= 32) return 11;
-    if (rows >= 1024 && nv <= 64) return 12;
-    if (nv <= 128) return 1;
-    if (nv <= 1024) return 2;
-    if (nv <= 2048) return 4;
-    return nv <= 4096 ? 8 : 0;
-}
-
-template <typename T, uint32_t ACT, bool UP>
-bool launch_glu_up(const GluArgs& a, cudaStream_t st) {
+template <typename T, bool UP>
+bool launch_glu(const GluArgs& a, cudaStream_t st) {
     if (vec_rows<T>(a.gate, a.ld_gate) && vec_rows<T>(a.up, a.ld_up) && vec_q<T>(a.q, a.ld_q))
-        LM_I8_VEC_ROWS(launch_glu_rows, T, ACT, UP);
-    LM_I8_ODD_ROWS(launch_glu_rows, T, ACT, UP);
-    glu_i8_kernel<T, ACT><<<a.rows, 256, 0, st>>>(a);
+        LM_I8_VEC_ROWS(false, launch_glu_rows, T, UP);
+    LM_I8_ODD_ROWS(launch_glu_rows, T, UP);
+    glu_i8_kernel<T><<<a.rows, 512, 0, st>>>(a);
     return LM_CUDA(cudaGetLastError());
-}
-template <typename T, uint32_t ACT>
-bool launch_glu_act(const GluArgs& a, cudaStream_t st) {
-    return a.up ? launch_glu_up<T, ACT, true>(a, st) : launch_glu_up<T, ACT, false>(a, st);
 }
 template <typename T>
 bool launch_glu(const GluArgs& a, cudaStream_t st) {
-    if (a.act == ACT_SILU) return launch_glu_act<T, ACT_SILU>(a, st);
-    if (a.act == ACT_GELU) return launch_glu_act<T, ACT_GELU>(a, st);
-    return launch_glu_act<T, LLAMINI_ACT_NONE>(a, st);
+    return a.up ? launch_glu<T, true>(a, st) : launch_glu<T, false>(a, st);
 }
+
 template <typename T, bool RESID>
 bool launch_norm(const NormArgs& a, cudaStream_t st) {
     if (vec_rows<T>(a.x, a.ld_x) && vec_rows<T>(a.resid, a.ld_resid) && vec_rows<T>(a.sum, a.ld_sum) && vec_q<T>(a.q, a.ld_q))
-        LM_I8_VEC_ROWS(launch_norm_rows, T, RESID);
+        LM_I8_VEC_ROWS(true, launch_norm_rows, T, RESID);
     LM_I8_ODD_ROWS(launch_norm_rows, T, RESID);
-    norm_i8_kernel<T><<<a.rows, 256, 0, st>>>(a);
+    norm_i8_kernel<T><<<a.rows, 512, 0, st>>>(a);
     return LM_CUDA(cudaGetLastError());
 }
 template <typename T>
