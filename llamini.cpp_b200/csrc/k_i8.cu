@@ -15,9 +15,10 @@ namespace {
 
 constexpr uint32_t kWarpRows = 8;          // rows at a time of a CTA whose warps have one each
 // The most threads of a CTA that keeps up to V pieces of E elements a thread in
-// registers, and whether the next row's pieces fit there too.
-template <bool WARP, uint32_t E, uint32_t V> constexpr uint32_t rows_threads() {
-    return WARP ? 32 * kWarpRows : V * E <= 8 || E == 1 ? 1024 : 512;
+// registers (1024 up to N elements, 16 without a norm's weights beside them), and
+// whether the next row's pieces fit there too.
+template <bool WARP, uint32_t E, uint32_t V, uint32_t N> constexpr uint32_t rows_threads() {
+    return WARP ? 32 * kWarpRows : V * E <= N || E == 1 ? 1024 : 512;
 }
 template <uint32_t E, uint32_t V> constexpr bool rows_ahead() { return V * E <= (E == 1 ? 8 : 32); }
 
@@ -68,7 +69,7 @@ __global__ void __launch_bounds__(512) norm_i8_kernel(const NormArgs a) {
 // h w of every element is kept from the first pass to the second. CTAs walk the
 // rows with w in registers and the next row's loads in flight.
 template <typename T, bool RESID, bool WARP, uint32_t E, uint32_t V>
-__global__ void __launch_bounds__(rows_threads<WARP, E, V>()) norm_i8_rows_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(rows_threads<WARP, E, V, 8>()) norm_i8_rows_kernel(const NormArgs a) {
     constexpr uint32_t R = WARP ? kWarpRows : 1;     // rows of a CTA at a time
     constexpr bool AHEAD = rows_ahead<E, V>();
     __shared__ uint32_t red[WARP ? 1 : 128];
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(512) glu_i8_kernel(const GluArgs a) {
 // The same with a row's values in the registers of G threads, read and
 // activated once; the next row's loads are in flight meanwhile.
 template <typename T, bool UP, bool WARP, uint32_t E, uint32_t V>
-__global__ void __launch_bounds__(rows_threads<WARP, E, V>()) glu_i8_rows_kernel(const GluArgs a) {
+__global__ void __launch_bounds__(rows_threads<WARP, E, V, 16>(), V * E == 24 && V == 3 ? 2 : 1) glu_i8_rows_kernel(const GluArgs a) {
     constexpr uint32_t R = WARP ? kWarpRows : 1;
     constexpr bool AHEAD = rows_ahead<E, V>();
     __shared__ uint32_t red[WARP ? 1 : 128];
@@ -644,13 +645,14 @@ bool launch_glu_rows(const GluArgs& a, const RowShape& r, cudaStream_t st) {
 // path through a row; long ones enough threads for two CTAs an SM and no idle lanes
 // in the last round. us of bf16 norm with residual at V = 1, 2, 4: 4096 x 2048
 // 11.8, 12.6, 13.1; 4096 x 4096 21.7, 22.6, 21.1. bf16 SiLU at V = 2, 3, 4: 4096 x
-// 4864 19.4, 22.7, 20.8; 4096 x 11008 (3, 4, 6) 47.0, 51.2, 46.9; f32 (6, 8) 63.2, 68.5.
+// 4864 19.4, 22.7, 20.8; 4096 x 11008 (3, 4, 6) 42.6, 51.2, 46.9; f32 (6, 8) 63.2, 68.5.
 // Many short rows, a warp each: 20000 x 128 bf16 norm 8.2 against 10.1 us.
 uint32_t rows_vectors(bool norm, uint32_t rows, uint32_t nv) {
     if (rows >= 1024 && nv <= 32) return 11;
     if (rows >= 1024 && nv <= 64) return 12;
     if (nv <= 256) return 1;
     if (nv <= 1024) return norm && rows >= 1024 && nv >= 512 ? 4 : 2;
+    if (!norm && rows < 1024 && nv <= 2048) return 2;
     if (nv <= 1536) return 3;
     if (nv <= 2048) return 4;
     return nv <= 3072 ? 6 : nv <= 4096 ? 8 : 0;
