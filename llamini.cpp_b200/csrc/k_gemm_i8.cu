@@ -423,15 +423,15 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 2) gemm_i8_few_kernel(const
 // holding 128 of the tokens' rows and half of the channels' rows in shared
 // memory; one thread of the pair's first CTA issues MMAs that read both
 // (cta_group::2, M = 256) and leave each CTA its 128 tokens' sums in its own
-// tensor memory. Two accumulators alternate, so the epilogue of a tile (eight
+// tensor memory. Two accumulators alternate, so the epilogue of a tile (four
 // warps: tensor memory -> scales -> shared memory -> TMA store) runs under the
 // next tile's MMAs. Persistent: one pair per two SMs walks the tiles. When the
 // last round has work for at most half of the pairs, its tiles are halved to
 // 128 channels, so that more of them share it.
 struct Many {
     static constexpr uint32_t kA = 128 * kSlab, kB = 64 * kSlab, kStage = kA + 2 * kB;
-    static constexpr uint32_t kStages = 5;
-    static constexpr uint32_t kEpi = 8;               // epilogue warps
+    static constexpr uint32_t kStages = 6;
+    static constexpr uint32_t kEpi = 4;               // epilogue warps
     static constexpr uint32_t kOut = 4096;            // 32 tokens x 128 bytes of outputs, one a warp
     static constexpr uint32_t kThreads = (kEpi + 2) * 32;
     static constexpr size_t kSmem = kStage * kStages + kEpi * kOut + 2 * 256 * 4 + 1024;
@@ -460,16 +460,26 @@ __device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
                  ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
 }
-__device__ __forceinline__ void tmem_get32(uint32_t taddr, int* r) {
+// 32 columns of this warp's 32 tensor-memory lanes; the registers are valid
+// after tmem_wait32, which every use has to follow.
+__device__ __forceinline__ void tmem_load32(uint32_t taddr, int* r) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
                  " %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
-                 "tcgen05.wait::ld.sync.aligned;\n"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
                    "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
                    "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
                    "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(taddr) : "memory");
 }
+__device__ __forceinline__ void tmem_wait32(int* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :: "memory");
+}
+
 // The tile a pair works on at step t: groups of up to 8 token tiles, within
 // a group the token tile changes fastest, so that the tiles in flight share
 // rows of both operands in L2. From step `whole` on, two steps to a tile.
@@ -590,57 +600,68 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
         }
     } else {
         constexpr uint32_t kCw = 128 / sizeof(T);    // channels of a staged chunk
-        const uint32_t quad = warp & 3u, side = warp >> 2;   // tensor-memory lanes; half of the tile's channels
         float* const sw = reinterpret_cast<float*>(sm + M::kStage * M::kStages + M::kEpi * M::kOut);
         float* const sb = sw + 256;
         uint8_t* const out = sm + M::kStage * M::kStages + warp * M::kOut;
         uint32_t acc = 0;
         bool bad = false;
         // the scales of a tile are loaded while the tile before is finished
-        float ws_next = 0.f, b_next = 0.f, as_next = 0.f;
+        float ws_next[2] = {}, b_next[2] = {}, as_next = 0.f;
         auto load_scales = [&](uint32_t t) {
             if (t >= tiles.steps) return;
             const ManyTile q = tile_at(t, tiles);
-            const uint32_t n = q.n0 + threadIdx.x, r = q.tm * 256 + rank * 128 + quad * 32 + lane;
-            ws_next = n < g.n ? g.ws[n] : 0.f;
-            b_next = g.bias && n < g.n ? g.bias[n] : 0.f;
+            const uint32_t r = q.tm * 256 + rank * 128 + warp * 32 + lane;
+#pragma unroll
+            for (uint32_t h = 0; h < 2; h++) {
+                const uint32_t n = q.n0 + h * 128 + threadIdx.x;
+                ws_next[h] = n < g.n ? g.ws[n] : 0.f;
+                b_next[h] = g.bias && n < g.n ? g.bias[n] : 0.f;
+            }
             as_next = r < g.m ? g.as[r] : 0.f;
         };
         load_scales(pair);
         for (uint32_t t = pair; t < tiles.steps; t += pairs) {
             const ManyTile q = tile_at(t, tiles);
             if (q.n0 >= g.n) break;                  // (only ever the last step)
-            const uint32_t buf = acc & 1u, r0 = q.tm * 256 + rank * 128 + quad * 32;
-            asm volatile("bar.sync 1, 256;\n" ::: "memory");      // the tile before has read its scales
-            sw[threadIdx.x] = ws_next;
-            sb[threadIdx.x] = b_next;
+            const uint32_t buf = acc & 1u, r0 = q.tm * 256 + rank * 128 + warp * 32;
+            const uint32_t ta = tmem + ((warp * 32u) << 16) + buf * 256, cols = min(q.bn, g.n - q.n0);
+            asm volatile("bar.sync 1, 128;\n" ::: "memory");      // the tile before has read its scales
+#pragma unroll
+            for (uint32_t h = 0; h < 2; h++) {
+                sw[h * 128 + threadIdx.x] = ws_next[h];
+                sb[h * 128 + threadIdx.x] = b_next[h];
+            }
             const float as = as_next;
             load_scales(t + pairs);
-            asm volatile("bar.sync 1, 256;\n" ::: "memory");
+            asm volatile("bar.sync 1, 128;\n" ::: "memory");
             bad |= !bar_wait_long(&S.accf[buf], (acc / 2) & 1u, &S.abort);
             bad = __any_sync(0xffffffffu, bad);
             tc_after();
-            const uint32_t c0 = side * (q.bn / 2), left = g.n - q.n0;
-            const uint32_t c1 = min(c0 + q.bn / 2, left);
-            for (uint32_t c = c0; c < c1; c += kCw) {
-                uint4 p[8];                          // this token's 128 bytes
+            // 32 channels at a time, the next 32 on their way from tensor memory
+            int v[2][32];
+            uint4 p[8];                              // this token's 128 bytes
+            tmem_load32(ta, v[0]);
+#pragma unroll 1
+            for (uint32_t c2 = 0; c2 < cols; c2 += 64) {
 #pragma unroll
-                for (uint32_t h = 0; h < kCw / 32; h++) {
-                    int v[32];
-                    tmem_get32(tmem + ((quad * 32u) << 16) + buf * 256 + c + h * 32, v);
+                for (uint32_t h = 0; h < 2; h++) {
+                    const uint32_t c = c2 + h * 32;  // (32 columns past `cols` may be read, and are not stored)
+                    if (h == 1 && c >= cols && kCw == 32) break;
+                    tmem_wait32(v[h]);
+                    if (c + 32 < cols || (kCw == 64 && h == 0)) tmem_load32(ta + c + 32, v[h ^ 1]);
                     float y[32];
 #pragma unroll
                     for (uint32_t i = 0; i < 32; i += 4) {
-                        const float4 w4 = *reinterpret_cast<const float4*>(sw + c + h * 32 + i);
-                        y[i] = (float)v[i] * as * w4.x;
-                        y[i + 1] = (float)v[i + 1] * as * w4.y;
-                        y[i + 2] = (float)v[i + 2] * as * w4.z;
-                        y[i + 3] = (float)v[i + 3] * as * w4.w;
+                        const float4 w4 = *reinterpret_cast<const float4*>(sw + c + i);
+                        y[i] = (float)v[h][i] * as * w4.x;
+                        y[i + 1] = (float)v[h][i + 1] * as * w4.y;
+                        y[i + 2] = (float)v[h][i + 2] * as * w4.z;
+                        y[i + 3] = (float)v[h][i + 3] * as * w4.w;
                     }
                     if (g.bias) {
 #pragma unroll
                         for (uint32_t i = 0; i < 32; i += 4) {
-                            const float4 b4 = *reinterpret_cast<const float4*>(sb + c + h * 32 + i);
+                            const float4 b4 = *reinterpret_cast<const float4*>(sb + c + i);
                             y[i] += b4.x; y[i + 1] += b4.y; y[i + 2] += b4.z; y[i + 3] += b4.w;
                         }
                     }
@@ -658,35 +679,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
                         for (uint32_t u = 0; u < 4; u++)
                             p[h * 4 + u] = make_uint4(pack2(y[8 * u], y[8 * u + 1], T()), pack2(y[8 * u + 2], y[8 * u + 3], T()),
                                                       pack2(y[8 * u + 4], y[8 * u + 5], T()), pack2(y[8 * u + 6], y[8 * u + 7], T()));
+                        if (h == 0) continue;
                     }
-                }
-                if (TMA_OUT && lane == 0)            // the store before has read the buffer
-                    asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
-                __syncwarp();
-                // 16-byte unit u of a token's 128 bytes lies at u ^ (token % 8)
-#pragma unroll
-                for (uint32_t u = 0; u < 8; u++)
-                    *reinterpret_cast<uint4*>(out + lane * 128 + ((u ^ (lane & 7u)) << 4)) = p[u];
-                if (TMA_OUT) {
-                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    const uint32_t n = q.n0 + (kCw == 32 ? c : c2);       // first channel of the chunk
+                    if (TMA_OUT && lane == 0)        // the store before has read the buffer
+                        asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) {
-                        if (r0 < g.m)
-                            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n"
-                                         ::"l"(reinterpret_cast<uint64_t>(&map_o)), "r"(q.n0 + c), "r"(r0),
-                                           "r"(smem_u32(out)) : "memory");
-                        asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
-                    }
-                } else {
-                    __syncwarp();
-                    constexpr uint32_t per = 4 / sizeof(T);       // elements of a lane's word
-                    const uint32_t n = q.n0 + c + lane * per;
-                    for (uint32_t r = 0; r < 32 && r0 + r < g.m; r++) {
-                        const T* word = reinterpret_cast<const T*>(out + r * 128 + (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4);
-                        T* dst = static_cast<T*>(g.out) + (uint64_t)(r0 + r) * g.ld_out + n;
+                    // 16-byte unit u of a token's 128 bytes lies at u ^ (token % 8)
 #pragma unroll
-                        for (uint32_t e = 0; e < per; e++)
-                            if (n + e < g.n) dst[e] = word[e];
+                    for (uint32_t u = 0; u < 8; u++)
+                        *reinterpret_cast<uint4*>(out + lane * 128 + ((u ^ (lane & 7u)) << 4)) = p[u];
+                    if (TMA_OUT) {
+                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (r0 < g.m)
+                                asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n"
+                                             ::"l"(reinterpret_cast<uint64_t>(&map_o)), "r"(n), "r"(r0), "r"(smem_u32(out)) : "memory");
+                            asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+                        }
+                    } else {
+                        __syncwarp();
+                        constexpr uint32_t per = 4 / sizeof(T);   // elements of a lane's word
+                        const uint32_t nl = n + lane * per;
+                        for (uint32_t r = 0; r < 32 && r0 + r < g.m; r++) {
+                            const T* word = reinterpret_cast<const T*>(out + r * 128 + (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4);
+                            T* dst = static_cast<T*>(g.out) + (uint64_t)(r0 + r) * g.ld_out + nl;
+#pragma unroll
+                            for (uint32_t e = 0; e < per; e++)
+                                if (nl + e < g.n) dst[e] = word[e];
+                        }
                     }
                 }
             }
