@@ -702,12 +702,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
                         __syncwarp();
                         constexpr uint32_t per = 4 / sizeof(T);   // elements of a lane's word
                         const uint32_t nl = n + lane * per;
-                        for (uint32_t r = 0; r < 32 && r0 + r < g.m; r++) {
-                            const T* word = reinterpret_cast<const T*>(out + r * 128 + (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4);
+#pragma unroll 8
+                        for (uint32_t r = 0; r < 32; r++) {
+                            const uint32_t w = *reinterpret_cast<const uint32_t*>(out + r * 128 + (((lane >> 2) ^ (r & 7u)) << 4) +
+                                                                                  (lane & 3u) * 4);
+                            if (r0 + r >= g.m) continue;
+                            const T* e = reinterpret_cast<const T*>(&w);
                             T* dst = static_cast<T*>(g.out) + (uint64_t)(r0 + r) * g.ld_out + nl;
 #pragma unroll
-                            for (uint32_t e = 0; e < per; e++)
-                                if (nl + e < g.n) dst[e] = word[e];
+                            for (uint32_t i = 0; i < per; i++)
+                                if (nl + i < g.n) dst[i] = e[i];
                         }
                     }
                 }
