@@ -102,6 +102,100 @@ bool launch_any(const GemmI8Args& g, cudaStream_t st) {
     return LM_CUDA(cudaGetLastError());
 }
 
+// One to eight tokens, the products of single-sequence decoding: each warp
+// streams R channels' rows, 16 bytes a lane and up to 4 R loads in flight, against
+// M tokens' rows in shared memory. dp4a keeps up with the memory (M / 4 of them a
+// weight byte), there is nothing to set up, and no SM waits for another.
+constexpr uint32_t kVecWarps = 8;
+constexpr uint32_t kVecSmem = 44 * 1024;         // most bytes of the tokens' rows
+
+template <typename T, uint32_t M, uint32_t R>
+__global__ void __launch_bounds__(32 * kVecWarps) gemv_i8_kernel(const GemmI8Args g) {
+    extern __shared__ __align__(16) uint8_t sm_raw[];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t nv = g.k / 16;                    // 16-byte vectors of a row
+    const uint32_t n0 = (blockIdx.x * kVecWarps + warp) * R;
+    pdl_trigger();
+    pdl_wait();
+    uint4* const sa = reinterpret_cast<uint4*>(sm_raw);
+    for (uint32_t i = threadIdx.x; i < M * nv; i += 32 * kVecWarps) {
+        const uint32_t m = i / nv, v = i - m * nv;
+        sa[i] = m < g.m ? *(reinterpret_cast<const uint4*>(g.a + (uint64_t)m * g.ld_a) + v) : make_uint4(0, 0, 0, 0);
+    }
+    const uint4* w[R];                               // rows past the last channel read the last one's again
+#pragma unroll
+    for (uint32_t r = 0; r < R; r++) w[r] = reinterpret_cast<const uint4*>(g.w + (uint64_t)min(n0 + r, g.n - 1) * g.ld_w);
+    constexpr uint32_t U = 4;                        // vectors of a row in flight in a lane
+    uint4 x[U][R];
+    auto load = [&](uint32_t v0) {
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++)
+#pragma unroll
+            for (uint32_t r = 0; r < R; r++) {
+                const uint32_t v = v0 + u * 32 + lane;
+                x[u][r] = v < nv ? __ldcs(w[r] + v) : make_uint4(0, 0, 0, 0);
+            }
+    };
+    load(0);
+    __syncthreads();
+    int acc[R][M] = {};
+    for (uint32_t v0 = 0; v0 < nv; v0 += U * 32) {
+        if (v0) load(v0);
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) {
+            const uint32_t v = min(v0 + u * 32 + lane, nv - 1);           // (the weights there are zero)
+#pragma unroll
+            for (uint32_t m = 0; m < M; m++) {
+                const uint4 a = sa[m * nv + v];
+#pragma unroll
+                for (uint32_t r = 0; r < R; r++) {
+                    acc[r][m] = __dp4a((int)x[u][r].x, (int)a.x, acc[r][m]);
+                    acc[r][m] = __dp4a((int)x[u][r].y, (int)a.y, acc[r][m]);
+                    acc[r][m] = __dp4a((int)x[u][r].z, (int)a.z, acc[r][m]);
+                    acc[r][m] = __dp4a((int)x[u][r].w, (int)a.w, acc[r][m]);
+                }
+            }
+        }
+    }
+    // lane r M + m finishes token m of channel r
+    int mine = 0;
+#pragma unroll
+    for (uint32_t r = 0; r < R; r++)
+#pragma unroll
+        for (uint32_t m = 0; m < M; m++) {
+            const int s = __reduce_add_sync(0xffffffffu, acc[r][m]);
+            if (lane == r * M + m) mine = s;
+        }
+    const uint32_t m = lane % M, n = n0 + lane / M;
+    if (lane < R * M && m < g.m && n < g.n) {
+        float y = (float)mine * g.as[m] * g.ws[n];
+        if (g.bias) y += g.bias[n];
+        static_cast<T*>(g.out)[(uint64_t)m * g.ld_out + n] = from_f32<T>(y);
+    }
+}
+
+template <typename T, uint32_t M, uint32_t R>
+bool launch_vec(const GemmI8Args& g, cudaStream_t st) {
+    const uint32_t per = kVecWarps * R;
+    return LM_CUDA(launch_k(gemv_i8_kernel<T, M, R>, dim3((g.n + per - 1) / per), dim3(32 * kVecWarps), (size_t)M * g.k, st, g));
+}
+// Two channels a warp where there are enough for every SM, else one (one token
+// x 5632 x 2048: 2.9 us with one, 3.3 with two; 22016 x 4096: 16.1, 15.5).
+template <typename T, uint32_t M>
+bool launch_vec(const GemmI8Args& g, cudaStream_t st) {
+    return M == 8 || g.n > 8192 ? launch_vec<T, M, 2>(g, st) : launch_vec<T, M, 1>(g, st);
+}
+// Whether the vectors' kernel is the fastest: up to two tokens always (one token x
+// 4096 x 4096: 4.7 us against the tensor cores' 6.9; 32000 x 2048 10.9, 12.8), more
+// while their rows are short (four x 4096 x 4096 5.9 against 7.5, x 11008 16.3
+// against 12.0; eight x 2560 x 2048 3.4 against 6.2, 12288 x 4096 15.5 against 12.8).
+bool vec_wins(const GemmI8Args& g) {
+    if (g.k % 16 != 0 || g.m > 8) return false;
+    const uint32_t M = g.m <= 2 ? g.m : g.m <= 4 ? 4 : 8;
+    if ((uint64_t)M * g.k > kVecSmem) return false;
+    return M <= 2 || (M == 4 ? g.k <= 5120 : g.k <= 4096 && g.n <= 4096);
+}
+
 // ---------------------------------------------------------------- tensor cores
 
 constexpr uint32_t kSlab = 128;                  // columns (bytes) of both operands in a stage
@@ -882,6 +976,9 @@ bool tma_rows(const GemmI8Args& g) {
 template <typename T>
 bool launch(const GemmI8Args& g, cudaStream_t st) {
     if (!tma_rows(g)) return launch_any<T>(g, st);
+    if (vec_wins(g))
+        return g.m == 1 ? launch_vec<T, 1>(g, st) : g.m == 2 ? launch_vec<T, 2>(g, st)
+             : g.m <= 4 ? launch_vec<T, 4>(g, st) : launch_vec<T, 8>(g, st);
     const uint64_t tn = (g.n + 127) / 128, sms = i8_sms();
     const uint32_t nkb = (g.k + kSlab - 1) / kSlab;
     const uint64_t wide = 6 * sms / 5, most = nkb < 30 ? wide : 3 * sms / 5;
