@@ -149,10 +149,16 @@ int llamini_glu_i8_device(u32 type, const void* d_gate, u64 ld_gate, const void*
 
 /* out[m][j] = (sum_k a[m][k] w[j][k]) * a_scale[m] * w_scale[j] (+ bias[j]) for
  * m < rows, j < n: the sum exact in 32-bit integers, the rest in f32, rounded to
- * out_type (F32, F16, BF16). d_bias may be NULL. a is rows x cols, w n x cols. */
+ * out_type (F32, F16, BF16). d_bias may be NULL. a is rows x cols, w n x cols. An
+ * output's bits do not depend on the other rows or channels of the call. */
 int llamini_gemm_i8_device(const i8* d_a, u64 ld_a, const f32* d_a_scale, u32 rows,
                            const i8* d_w, u64 ld_w, const f32* d_w_scale, u32 n, u32 cols,
                            const f32* d_bias, u32 out_type, void* d_out, u64 ld_out, void* stream);
+
+/* Waits for `stream`, then 0, or -1 when a bounded wait (2 s) inside a product's
+ * kernel has run out on the current device since the last call: the outputs it
+ * was for are NaN. Not during a stream capture. */
+int llamini_i8_status(void* stream);
 
 /* ---- device-resident decoding sessions (generate.c:122-167 without host
  *      round trips) --------------------------------------------------------- */

@@ -30,6 +30,10 @@ struct GemmI8Args {
     uint32_t m, n, k;
 };
 
+// A sum with its scales and bias, each product and sum rounded on its own, so
+// that an output is the same whichever kernel and tile it comes from.
+__device__ __forceinline__ float scaled(int sum, float as, float ws) { return __fmul_rn(__fmul_rn((float)sum, as), ws); }
+
 // Rows of any pitch and alignment: 64 x 64 outputs a CTA, 64 columns of both
 // operands at a time in shared memory as words of four, dp4a on 4 x 4 outputs
 // a thread.
@@ -84,8 +88,8 @@ __global__ void __launch_bounds__(256) gemm_i8_any_kernel(const GemmI8Args g) {
         for (uint32_t j = 0; j < 4; j++) {
             const uint32_t n = n0 + tx + 16 * j;
             if (n >= g.n) continue;
-            float v = (float)acc[i][j] * g.as[m] * g.ws[n];
-            if (g.bias) v += g.bias[n];
+            float v = scaled(acc[i][j], g.as[m], g.ws[n]);
+            if (g.bias) v = __fadd_rn(v, g.bias[n]);
             static_cast<T*>(g.out)[(uint64_t)m * g.ld_out + n] = from_f32<T>(v);
         }
     }
@@ -168,8 +172,8 @@ __global__ void __launch_bounds__(32 * kVecWarps) gemv_i8_kernel(const GemmI8Arg
         }
     const uint32_t m = lane % M, n = n0 + lane / M;
     if (lane < R * M && m < g.m && n < g.n) {
-        float y = (float)mine * g.as[m] * g.ws[n];
-        if (g.bias) y += g.bias[n];
+        float y = scaled(mine, g.as[m], g.ws[n]);
+        if (g.bias) y = __fadd_rn(y, g.bias[n]);
         static_cast<T*>(g.out)[(uint64_t)m * g.ld_out + n] = from_f32<T>(y);
     }
 }
@@ -476,8 +480,8 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 2) gemm_i8_few_kernel(const
             float y[4];
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++) {
-                y[i] = (float)x[i] * as * ws[i];
-                if (g.bias) y[i] += b[i];
+                y[i] = scaled(x[i], as, ws[i]);
+                if (g.bias) y[i] = __fadd_rn(y[i], b[i]);
             }
             store4<T>(g, m0 + t, n, y, vec);
         };
@@ -747,16 +751,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
 #pragma unroll
                     for (uint32_t i = 0; i < 32; i += 4) {
                         const float4 w4 = *reinterpret_cast<const float4*>(sw + c + i);
-                        y[i] = (float)v[h][i] * as * w4.x;
-                        y[i + 1] = (float)v[h][i + 1] * as * w4.y;
-                        y[i + 2] = (float)v[h][i + 2] * as * w4.z;
-                        y[i + 3] = (float)v[h][i + 3] * as * w4.w;
+                        y[i] = scaled(v[h][i], as, w4.x);
+                        y[i + 1] = scaled(v[h][i + 1], as, w4.y);
+                        y[i + 2] = scaled(v[h][i + 2], as, w4.z);
+                        y[i + 3] = scaled(v[h][i + 3], as, w4.w);
                     }
                     if (g.bias) {
 #pragma unroll
                         for (uint32_t i = 0; i < 32; i += 4) {
                             const float4 b4 = *reinterpret_cast<const float4*>(sb + c + i);
-                            y[i] += b4.x; y[i + 1] += b4.y; y[i + 2] += b4.z; y[i + 3] += b4.w;
+                            y[i] = __fadd_rn(y[i], b4.x);
+                            y[i + 1] = __fadd_rn(y[i + 1], b4.y);
+                            y[i + 2] = __fadd_rn(y[i + 2], b4.z);
+                            y[i + 3] = __fadd_rn(y[i + 3], b4.w);
                         }
                     }
                     if (bad) {
@@ -904,9 +911,10 @@ bool launch_few(const GemmI8Args& g, cudaStream_t st) {
     const uint32_t nkb = (g.k + kSlab - 1) / kSlab;
     // as many parts as leave two CTAs an SM and two stages a part (20 tiles of 16
     // stages: 6.2 us in one part, 4.7 in four or eight; 172 tiles of 32: 21.1 us in
-    // one part, 31.9 in two, which no longer run at once)
+    // one part, 31.9 in two, which no longer run at once); of clusters of eight, 32
+    // run at once (35 tiles of 38 stages: 11.9 us in eight parts, 7 in four)
     uint32_t cs = 1;
-    while (cs < 8 && tiles * cs * 2 <= 2 * i8_sms() && nkb / (cs * 2) >= 2) cs *= 2;
+    while (cs < 8 && tiles * cs * 2 <= (cs == 4 ? 256 : 2 * i8_sms()) && nkb / (cs * 2) >= 2) cs *= 2;
     if (tiles * cs > 0x7FFFFFFFull) {
         set_error("gemm_i8: %u x %u outputs are too many for one call", g.m, g.n);
         return false;
@@ -1028,4 +1036,20 @@ extern "C" int llamini_gemm_i8_device(const i8* d_a, u64 ld_a, const f32* d_a_sc
     const bool ok = out_type == GGML_TYPE_F32 ? launch<float>(g, st)
                   : out_type == GGML_TYPE_F16 ? launch<__half>(g, st) : launch<__nv_bfloat16>(g, st);
     return ok ? 0 : -1;
+}
+
+extern "C" int llamini_i8_status(void* stream) {
+    using namespace lm;
+    const void* none[1] = {nullptr};
+    if (!i8_device_ptrs("i8_status", none, 1)) return -1;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    uint32_t err = 0, zero = 0;
+    if (!LM_CUDA(cudaMemcpyFromSymbolAsync(&err, g_i8_err, sizeof(err), 0, cudaMemcpyDeviceToHost, st)) ||
+        !LM_CUDA(cudaStreamSynchronize(st)))
+        return -1;
+    if (err == 0) return 0;
+    set_error("gemm_i8: a wait inside a kernel ran out; the outputs it was for are NaN");
+    LM_CUDA(cudaMemcpyToSymbolAsync(g_i8_err, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, st));
+    LM_CUDA(cudaStreamSynchronize(st));
+    return -1;
 }

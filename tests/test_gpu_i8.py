@@ -451,6 +451,24 @@ def test_gemm_pitches_past_32_bits(gpu):
             assert torch.equal(out.double(), rows.double() @ rows.double().t())
 
 
+@pytest.mark.parametrize("type", [0, 1, 30])
+@pytest.mark.parametrize("n,k", [(300, 512), (896, 4864), (2048, 100)])
+def test_gemm_outputs_do_not_depend_on_the_batch(gpu, type, n, k):
+    """A token alone, in batches of every kernel and tile, and from rows of an
+    odd pitch: the same bits."""
+    g = _gen(n)
+    m = 1200
+    a, w = Rows(m, k, torch.int8, (-k) % 16, fill=_ints(g, m, k)), Rows(n, k, torch.int8, (-k) % 16, fill=_ints(g, n, k))
+    sa, sw, b = torch.rand(m, generator=g, device="cuda"), torch.rand(n, generator=g, device="cuda"), _rand(g, n, scale=100.0)
+    whole = Rows(m, n, DT[type])
+    _ok(gpu, _gemm(gpu, a, sa, w, sw, b, type, whole, m, n, k))
+    for rows in (1, 2, 3, 7, 16, 31, 64, 100, 200, 500):
+        for layout in (a, Rows(rows, k, torch.int8, 3, 1, a.t[:rows])):
+            out = Rows(rows, n, DT[type], pad=5 if rows % 2 else 0)
+            _ok(gpu, _gemm(gpu, layout, sa, w, sw, b, type, out, rows, n, k))
+            assert torch.equal(out.t, whole.t[:rows])
+
+
 # ---------------------------------------------------------------- together
 
 def _feed_forward(gpu, x, resid, w, gate_up, s_gu, down, s_d, act, type):
@@ -586,6 +604,11 @@ def test_calls_on_two_streams_at_once(gpu):
     for os_ in outs:
         for o, wo in zip(os_, want):
             assert torch.equal(o, wo)
+
+
+def test_no_wait_has_run_out(gpu):
+    """After every product above: no kernel has given up a wait."""
+    assert gpu.lib().llamini_i8_status(_stream()) == 0, gpu.last_error()
 
 
 def test_host_memory_is_refused(gpu):

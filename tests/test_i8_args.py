@@ -120,3 +120,12 @@ def test_memory_that_no_kernel_may_use_is_refused(lm, fn):
     want = "not memory of the current device" if L.llamini_device_count() > 0 else "no usable CUDA device"
     assert want in lm.last_error()
     L.llamini_clear_error()
+
+
+def test_status_without_a_device(lm):
+    L = lm.lib()
+    if L.llamini_device_count() > 0:
+        pytest.skip("a GPU is present")
+    assert L.llamini_i8_status(None) == -1
+    assert "no usable CUDA device" in lm.last_error()
+    L.llamini_clear_error()
