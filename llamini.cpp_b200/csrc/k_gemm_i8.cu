@@ -253,6 +253,9 @@ __device__ __forceinline__ void bar_drain(uint64_t* bar, uint32_t parity) {
     while (!bar_try(smem_u32(bar), parity) && now_ns() - t0 < kWaitNs) {
     }
 }
+__device__ __forceinline__ void map_prefetch(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 // Tile of `map` from column x, row y on into this CTA's shared memory.
 __device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n"
@@ -381,6 +384,10 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 2) gemm_i8_few_kernel(const
     const uint32_t nkb = (g.k + kSlab - 1) / kSlab;
     const uint32_t kb0 = (uint32_t)((uint64_t)nkb * rank / cs), kb1 = (uint32_t)((uint64_t)nkb * (rank + 1) / cs);
     pdl_trigger();
+    if (threadIdx.x == 32) {
+        map_prefetch(&map_w);
+        map_prefetch(&map_a);
+    }
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < F::kStages; i++) {
             mbar_init(&S.full[i], 1);
@@ -612,6 +619,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
     const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const uint32_t nkb = (g.k + kSlab - 1) / kSlab;
     pdl_trigger();
+    if (threadIdx.x == 32) {
+        map_prefetch(&map_w);
+        map_prefetch(&map_a);
+    }
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < M::kStages; i++) {
             mbar_init(&S.full[i], 1);
