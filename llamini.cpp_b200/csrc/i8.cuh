@@ -44,11 +44,7 @@ inline bool i8_device_ptrs(const char* who, const void* const* ptrs, int n) {
     for (int i = 0; i < n; i++) {
         if (!ptrs[i]) continue;
         cudaPointerAttributes a;
-        if (cudaPointerGetAttributes(&a, ptrs[i]) != cudaSuccess) {
-            cudaGetLastError();
-            set_error("%s: no usable CUDA device (this library has no CPU path)", who);
-            return false;
-        }
+        if (!LM_CUDA(cudaPointerGetAttributes(&a, ptrs[i]))) return false;
         if (a.type == cudaMemoryTypeManaged) continue;
         if (a.type != cudaMemoryTypeDevice || a.device != dev) {
             set_error("%s: pointer argument %d is not memory of the current device (%d)", who, i + 1, dev);

@@ -266,7 +266,6 @@ constexpr uint32_t kWRow = 96 * 1024;      // longest row that is staged whole
 constexpr uint32_t kWSlack = 64;           // behind it: the offset modulo 16, and words_at's read past a block
 constexpr uint32_t kWThreads = 256;
 
-
 // NW little-endian words from a 2-byte aligned address in shared memory (the
 // aligned words around it; reads up to two bytes past the range).
 template <int NW>
@@ -292,8 +291,9 @@ __device__ __forceinline__ float half_at(const uint8_t* p) {
 }
 
 // Elements 32 u .. 32 u + 31 of a row whose bytes (from the first block of
-// the staged segment on) are at `row`, in their own order, bit-identical to gguf.c:409-594:
-// each product and sum is rounded on its own.
+// the staged segment on) are at `row`, in their own order, bit-identical to
+// gguf.c:409-594: products and sums are rounded as there (a fused multiply-add
+// only where the product is exact).
 template <uint32_t T>
 __device__ __forceinline__ void unit_weights(const uint8_t* row, uint32_t u, float* y) {
     uint32_t w[8];
