@@ -192,14 +192,14 @@ bool launch_vec(const GemmI8Args& g, cudaStream_t st) {
     return M == 8 || g.n > 8192 ? launch_vec<T, M, 2>(g, st) : launch_vec<T, M, 1>(g, st);
 }
 // Whether the vectors' kernel is the fastest: up to two tokens always (one token x
-// 4096 x 4096: 4.7 us against the tensor cores' 6.9; 32000 x 2048 10.9, 12.8), more
-// while their rows are short (four x 4096 x 4096 5.9 against 7.5, x 11008 16.3
-// against 12.0; eight x 2560 x 2048 3.4 against 6.2, 12288 x 4096 15.5 against 12.8).
+// 4096 x 4096: 4.7 us against the tensor cores' 6.2; 32000 x 2048 10.9, 12.8), more
+// while their rows are short (four x 4096 x 4096 5.9 against 6.4, x 11008 16.3
+// against 10.8; eight x 2560 x 2048 3.4 against 4.5, 12288 x 4096 15.5 against 12.5).
 bool vec_wins(const GemmI8Args& g) {
     if (g.k % 16 != 0 || g.m > 8) return false;
     const uint32_t M = g.m <= 2 ? g.m : g.m <= 4 ? 4 : 8;
     if ((uint64_t)M * g.k > kVecSmem) return false;
-    return M <= 2 || (M == 4 ? g.k <= 5120 : g.k <= 4096 && g.n <= 4096);
+    return M <= 2 || (g.k <= 4096 && (M == 4 || g.n <= 4096));
 }
 
 // ---------------------------------------------------------------- tensor cores
@@ -372,8 +372,8 @@ __device__ __forceinline__ void store4(const GemmI8Args& g, uint32_t m, uint32_t
 // of the tokens. Nothing is left behind in global memory. Bound by the weights'
 // bytes for wide matrices (64 tokens x 22016 x 4096: 19.2 us, 4.85 TB/s with the
 // launch, of which the copies alone run at the memory's rate) and by the chain of
-// launch, first copy, cluster barrier and stores for small ones (16 tokens x 896 x
-// 896: 4.2 us).
+// launch, first copy, cluster barrier and stores for small ones (16 tokens x 1152 x
+// 896: 3.9 us).
 template <int NT>
 struct Few {
     static constexpr uint32_t kStage = kSlab * (128 + NT);
@@ -941,7 +941,7 @@ bool launch_few(const GemmI8Args& g, cudaStream_t st) {
     const uint64_t tiles_m = (g.m + NT - 1) / NT, tiles_n = (g.n + 127) / 128, tiles = tiles_m * tiles_n;
     const uint32_t nkb = (g.k + kSlab - 1) / kSlab;
     // as many parts as leave two CTAs an SM and two stages a part (20 tiles of 16
-    // stages: 6.2 us in one part, 4.7 in four or eight; 172 tiles of 32: 21.1 us in
+    // stages: 6.2 us in one part, 4.5 in four or eight; 172 tiles of 32: 21.1 us in
     // one part, 31.9 in two, which no longer run at once); of clusters of eight, 32
     // run at once (35 tiles of 38 stages: 11.9 us in eight parts, 7 in four)
     uint32_t cs = 1;
@@ -1006,13 +1006,13 @@ bool tma_rows(const GemmI8Args& g) {
 // Which kernel and tile. gemm_i8_few_kernel takes the narrowest token tile (16,
 // 32, 64, 128) that leaves no more than `most` tiles: more tiles are more SMs at
 // work, but each reads its channels' weights again; with long rows fewer tiles
-// and a deeper split of the columns win (64 tokens, 4096 x 4096: 16 wide 9.4 us,
-// 32 wide 8.8, 64 wide 10.3; 128 tokens, 4096 x 11008: 17.5, 15.4 at 64, 17.6 at
-// 128). Past 128 tokens, when even 128-wide tiles are more than that (or the rows
-// too short to split), gemm_i8_many_kernel: 512 tokens x 12288 x 4096 34.5 against 25.5 us, 256 x
-// 32000 x 2048 26.8 against 20.7; 512 x 4096 x 11008 the other way, 26.5 against
-// 28.1. Over 16 shapes x 19 token counts the choice costs 2.5 % on average over
-// the best of all tiles.
+// and a deeper split of the columns win (256 tokens x 1152 x 896: 64 wide 4.9 us, 128
+// wide 5.6; 160 tokens x 4096 x 11008: 64 wide 19.2, 128 wide 18.0). Past 128 tokens,
+// when even 128-wide tiles are more than that (or the rows too short to split),
+// gemm_i8_many_kernel: 512 tokens x 12288 x 4096 32.7 against 23.1 us, 256 x 32000 x
+// 2048 25.0 against 19.6; 256 x 4096 x 11008 the other way, 18.7 against 23.8. Over
+// 16 shapes x 19 token counts the choice costs 2.6 % on average over the best of
+// all tiles, and at most 24 %.
 template <typename T>
 bool launch(const GemmI8Args& g, cudaStream_t st) {
     if (!tma_rows(g)) return launch_any<T>(g, st);
