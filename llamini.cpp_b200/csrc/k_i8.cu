@@ -67,7 +67,10 @@ __global__ void __launch_bounds__(512) norm_i8_kernel(const NormArgs a) {
 
 // The same with a row in the registers of G threads (V vectors each), read once:
 // h w of every element is kept from the first pass to the second. CTAs walk the
-// rows with w in registers and the next row's loads in flight.
+// rows with w in registers and the next row's loads in flight. Bound by memory: bf16
+// 4096 x 4096 with residual and sum 20.9 us, 5.63 TB/s (two passes from L2 took 129
+// us with the conversion that follows, this 82), f32 2048 x 8192 34.3 us, 6.37 TB/s;
+// one row of 2048 1.8 us.
 template <typename T, bool RESID, bool WARP, uint32_t E, uint32_t V>
 __global__ void __launch_bounds__(rows_threads<WARP, E, V, 8>()) norm_i8_rows_kernel(const NormArgs a) {
     constexpr uint32_t R = WARP ? kWarpRows : 1;     // rows of a CTA at a time
@@ -190,7 +193,9 @@ __global__ void __launch_bounds__(512) glu_i8_kernel(const GluArgs a) {
 }
 
 // The same with a row's values in the registers of G threads, read and
-// activated once; the next row's loads are in flight meanwhile.
+// activated once; the next row's loads are in flight meanwhile. Bound by memory and
+// instruction issue (60 % of slots at bf16 4096 x 11008 SiLU: 42.6 us, 5.29 TB/s; f32
+// 2048 x 11008 32.8 us, 6.18 TB/s).
 template <typename T, bool UP, bool WARP, uint32_t E, uint32_t V>
 __global__ void __launch_bounds__(rows_threads<WARP, E, V, 16>(), V * E == 24 && V == 3 ? 2 : 1) glu_i8_rows_kernel(const GluArgs a) {
     constexpr uint32_t R = WARP ? kWarpRows : 1;
@@ -450,7 +455,9 @@ __global__ void __launch_bounds__(kWThreads) weights_i8_kernel(const WeightArgs 
 // The same for rows that fit: a CTA walks groups of rows (back to back in memory),
 // copies the next group's bytes while it works on this one's, and each thread
 // keeps the U units it decodes in registers from the maximum to the rounding. tpr
-// threads (whole warps) a row.
+// threads (whole warps) a row. Bound by instruction issue (13 an element, half of them
+// work of a row and thread): Q8_0 4096 x 11008 26.0 us, 3.58 TB/s; without its stores
+// 20.6, without its loads 23.0.
 __device__ __forceinline__ void copy16(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n"
                  ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");

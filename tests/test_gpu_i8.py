@@ -469,6 +469,68 @@ def test_gemm_outputs_do_not_depend_on_the_batch(gpu, type, n, k):
             assert torch.equal(out.t, whole.t[:rows])
 
 
+# ---------------------------------------------------------------- large and far
+
+@pytest.mark.parametrize("m,n,k", [(70001, 64, 64), (70001, 130, 48), (66000, 9, 33), (2, 140000, 64), (40, 140001, 64),
+                                   (300, 70000, 96)])
+def test_gemm_many_rows_or_channels(gpu, m, n, k):
+    _run_gemm(gpu, m, n, k, 0, True)
+
+
+@pytest.mark.parametrize("type", [0, 30])
+@pytest.mark.parametrize("cols", [8, 17, 300])
+def test_row_operators_many_rows(gpu, type, cols):
+    rows = 70001
+    g = _gen(cols)
+    x, r = Rows(rows, cols, DT[type], fill=_rand(g, rows, cols)), Rows(rows, cols, DT[type], fill=_rand(g, rows, cols))
+    w = 1 + _rand(g, cols, scale=0.05)
+    q, scale = Rows(rows, cols, torch.int8, (-cols) % 16), torch.empty(rows, device="cuda")
+    _ok(gpu, _norm(gpu, type, x, r, None, w, 1e-5, rows, cols, q, scale))
+    h = x.t.double() + r.t.double()
+    _check_int8(q.t, scale, h / (h.square().mean(1, True) + float(np.float32(1e-5))).sqrt() * w.double(), _norm_r(cols))
+    _ok(gpu, _glu(gpu, type, x, r, 0, rows, cols, q, scale))
+    _check_int8(q.t, scale, _act64(x.t.double(), 0) * r.t.double(), 20 * F24)
+    assert q.untouched_around()
+
+
+@pytest.mark.parametrize("cols", [64, 67, 4096])
+def test_pitches_past_32_bits(gpu, cols):
+    """Three rows 2.2 GB apart, of inputs and of int8 rows: offsets of rows
+    pass 32 bits in elements and in bytes."""
+    rows, far = 3, 2_200_000_000 // 64 * 64
+    g = _gen(cols)
+    buf = torch.empty(2 * far + 65536, dtype=torch.uint8, device="cuda")
+    x = _rand(g, rows, cols).half()
+    w = torch.ones(cols, device="cuda")
+    L = gpu.lib()
+    near_q, near_s = torch.empty(rows, 4096, dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+    far_s = torch.empty(rows, device="cuda")
+    xf = buf.view(torch.float16)
+    for i in range(rows):
+        xf[i * far // 2:i * far // 2 + cols] = x[i]
+    at_q = buf.data_ptr() + 32768
+    for run in (lambda p, ld, q, ldq, s: L.llamini_rms_norm_i8_device(1, p, ld, None, 0, None, 0, w.data_ptr(), 1e-5, rows, cols,
+                                                                      q, ldq, s.data_ptr(), _stream()),
+                lambda p, ld, q, ldq, s: L.llamini_glu_i8_device(1, p, ld, None, 0, 0, rows, cols, q, ldq, s.data_ptr(), _stream())):
+        _ok(gpu, run(x.data_ptr(), cols, near_q.data_ptr(), 4096, near_s))
+        _ok(gpu, run(buf.data_ptr(), far // 2, at_q, far, far_s))
+        assert torch.equal(near_s, far_s)
+        for i in range(rows):
+            assert torch.equal(buf[i * far + 32768:i * far + 32768 + cols].view(torch.int8), near_q[i, :cols])
+    # outputs of a product that far apart
+    a = _ints(g, rows, 64)
+    ones = torch.ones(cols, device="cuda")
+    b = _ints(g, cols, 64)
+    near = torch.empty(rows, cols, device="cuda")
+    _ok(gpu, L.llamini_gemm_i8_device(a.data_ptr(), 64, ones.data_ptr(), rows, b.data_ptr(), 64, ones.data_ptr(), cols, 64, None, 0,
+                                      near.data_ptr(), cols, _stream()))
+    _ok(gpu, L.llamini_gemm_i8_device(a.data_ptr(), 64, ones.data_ptr(), rows, b.data_ptr(), 64, ones.data_ptr(), cols, 64, None, 0,
+                                      buf.data_ptr(), far // 4, _stream()))
+    f = buf.view(torch.float32)
+    for i in range(rows):
+        assert torch.equal(f[i * far // 4:i * far // 4 + cols], near[i])
+
+
 # ---------------------------------------------------------------- together
 
 def _feed_forward(gpu, x, resid, w, gate_up, s_gu, down, s_d, act, type):
@@ -604,6 +666,65 @@ def test_calls_on_two_streams_at_once(gpu):
     for os_ in outs:
         for o, wo in zip(os_, want):
             assert torch.equal(o, wo)
+
+
+def test_weights_are_ready_for_the_product_behind_them(gpu, synth):
+    """Weights and product back to back on one stream, without a wait between
+    them, each time with other weights in the same buffers."""
+    n, k = 2048, 2048
+    rng = np.random.default_rng(3)
+    raws = [torch.from_numpy(synth.random_blocks(rng, 8, n * k).copy()).cuda() for _ in range(3)]
+    q, s = torch.empty(n, k, dtype=torch.int8, device="cuda"), torch.empty(n, device="cuda")
+    L, st = gpu.lib(), _stream()
+    for m in (1, 16, 700):
+        a, sa = _ints(_gen(m), m, k), torch.ones(m, device="cuda")
+        want, outs = [], []
+        for wait in (True, False):
+            for raw in raws * 3:
+                out = torch.empty(m, n, device="cuda")
+                _ok(gpu, L.llamini_weights_i8_device(8, raw.data_ptr(), n, k, q.data_ptr(), k, s.data_ptr(), st))
+                if wait:
+                    torch.cuda.synchronize()
+                _ok(gpu, L.llamini_gemm_i8_device(a.data_ptr(), k, sa.data_ptr(), m, q.data_ptr(), k, s.data_ptr(), n, k, None, 0,
+                                                  out.data_ptr(), n, st))
+                (want if wait else outs).append(out)
+        torch.cuda.synchronize()
+        for x, y in zip(want, outs):
+            assert torch.equal(x, y)
+
+
+def test_calls_from_two_host_threads(gpu):
+    """Each thread on a stream of its own, the same products at once."""
+    import threading
+    g = _gen(4)
+    shapes = [(1, 512, 1024), (20, 900, 640), (300, 512, 384), (5, 100, 77)]
+    jobs = []
+    for m, n, k in shapes:
+        kp = (k + 15) // 16 * 16
+        jobs.append((m, n, k, kp, _ints(g, m, kp), _ints(g, n, kp), torch.rand(m, generator=g, device="cuda"),
+                     torch.rand(n, generator=g, device="cuda")))
+    L = gpu.lib()
+    outs = [[torch.empty(j[0], j[1], device="cuda") for j in jobs] for _ in range(3)]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(t):
+        for _ in range(30):
+            for (m, n, k, kp, a, w, sa, sw), o in zip(jobs, outs[t]):
+                if L.llamini_gemm_i8_device(a.data_ptr(), kp, sa.data_ptr(), m, w.data_ptr(), kp, sw.data_ptr(), n, k, None, 0,
+                                            o.data_ptr(), n, streams[t].cuda_stream) != 0:
+                    failed.append(gpu.last_error())
+    threads = [threading.Thread(target=work, args=(t,)) for t in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed[0]
+    for (m, n, k, kp, a, w, sa, sw), x, y, z in zip(jobs, *outs):
+        _check_gemm(x, 0, a[:, :k], sa, w[:, :k], sw, None)
+        assert torch.equal(x, y) and torch.equal(x, z)
 
 
 def test_no_wait_has_run_out(gpu):
