@@ -112,8 +112,8 @@ int llamini_causal_mha_noalloc(const f32* d_q, const f32* d_key, const f32* d_va
  * uses scratch, so calls may overlap in time and may be captured into graphs.
  * Matrices are row-major; a pitch ld_* counts elements from row to row and is at
  * least the row's length. What lies between a row's end and the next row's start
- * is neither read nor written. Pitches in multiples of 16 elements from a 16-byte
- * aligned base are what the fast kernels take; other ones work, slower. 1 to
+ * is not written, and its values do not matter. Pitches in multiples of 16 elements
+ * from a 16-byte aligned base are what the fast kernels take; other ones work, slower. 1 to
  * 131071 columns; rows = 0 is a call without work. Outputs must not overlap
  * inputs, but for the sum of llamini_rms_norm_i8_device. */
 

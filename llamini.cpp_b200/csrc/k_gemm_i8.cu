@@ -36,8 +36,8 @@ __device__ __forceinline__ float scaled(int sum, float as, float ws) { return __
 
 // Rows of any pitch and alignment: 64 x 64 outputs a CTA, 64 columns of both
 // operands at a time in shared memory as words of four, dp4a on 4 x 4 outputs
-// a thread. For the calls that TMA and 16-byte loads cannot take; bound by dp4a and
-// byte loads (4096 x 4096 x 11008: 6.5 ms, 57 TOP/s).
+// a thread. For more than 8 tokens where TMA cannot read the rows; bound by dp4a
+// and byte loads (4096 x 4096 x 11008: 6.5 ms, 57 TOP/s).
 constexpr uint32_t kST = 64, kSW = kST / 4, kSPad = kSW + 1;
 
 __device__ __forceinline__ void load_words(uint32_t (*dst)[kSPad], const int8_t* src, uint64_t ld, uint32_t r0,
@@ -111,36 +111,74 @@ bool launch_any(const GemmI8Args& g, cudaStream_t st) {
 // streams R channels' rows, 16 bytes a lane and up to 4 R loads in flight, against
 // M tokens' rows in shared memory. dp4a keeps up with the memory (M / 4 of them a
 // weight byte), there is nothing to set up, and no SM waits for another. One token
-// x 22016 x 4096: 15.5 us, 5.8 TB/s, 89 % of the copy bandwidth; x 2560 x 2048: 2.3 us.
+// x 22016 x 4096: 15.6 us, 5.8 TB/s, 89 % of the copy bandwidth; x 2560 x 2048: 2.3 us;
+// rows at odd addresses, x 4096 x 4095: 8.2 us (the tiled kernel above: 142).
 constexpr uint32_t kVecWarps = 8;
 constexpr uint32_t kVecSmem = 44 * 1024;         // most bytes of the tokens' rows
 
-template <typename T, uint32_t M, uint32_t R>
+// The first n < 16 bytes at p, the rest zero; n = 16 takes any alignment.
+__device__ __noinline__ uint4 bytes16(const uint8_t* p, uint32_t n) {
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (uint32_t i = 0; i < 16; i++)
+        if (i < n) w[i >> 2] |= (uint32_t)p[i] << (8 * (i & 3u));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// How rows lie: 16-byte vectors throughout; aligned with a last vector cut
+// short; at any address.
+enum RowsAt : uint32_t { ROWS_WHOLE, ROWS_TAIL, ROWS_ANY };
+// Vector v (16 bytes) of a row of k bytes, read once by the device (STREAM: the
+// weights) or by every CTA: zeros past its end. Nothing behind the
+// row is read; a row at any address is read in the aligned words around the
+// vector, up to 3 bytes before the row's own first.
+template <uint32_t AT, bool STREAM>
+__device__ __forceinline__ uint4 row_vec(const uint8_t* row, uint32_t v, uint32_t k) {
+    const uint32_t at = 16 * v;
+    const uint8_t* p = row + at;
+    if (AT == ROWS_ANY) {
+        if (at + 19 <= k) {
+            const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+            const uint32_t* b = reinterpret_cast<const uint32_t*>(a & ~uintptr_t(3));
+            const uint32_t s = (uint32_t)(a & 3u) * 8u;
+            uint32_t w[5];
+#pragma unroll
+            for (uint32_t i = 0; i < 5; i++) w[i] = b[i];
+            return make_uint4(__funnelshift_r(w[0], w[1], s), __funnelshift_r(w[1], w[2], s), __funnelshift_r(w[2], w[3], s),
+                              __funnelshift_r(w[3], w[4], s));
+        }
+    } else {
+        if (at + 16 <= k) return STREAM ? __ldcs(reinterpret_cast<const uint4*>(p)) : *reinterpret_cast<const uint4*>(p);
+    }
+    return AT != ROWS_WHOLE && at < k ? bytes16(p, min(16u, k - at)) : make_uint4(0, 0, 0, 0);
+}
+
+template <typename T, uint32_t M, uint32_t R, uint32_t AT>
 __global__ void __launch_bounds__(32 * kVecWarps) gemv_i8_kernel(const GemmI8Args g) {
     extern __shared__ __align__(16) uint8_t sm_raw[];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    const uint32_t nv = g.k / 16;                    // 16-byte vectors of a row
+    const uint32_t nv = (g.k + 15) / 16;             // 16-byte vectors of a row
     const uint32_t n0 = (blockIdx.x * kVecWarps + warp) * R;
     pdl_trigger();
     pdl_wait();
     uint4* const sa = reinterpret_cast<uint4*>(sm_raw);
+#pragma unroll(M > 2 ? 4 : 1)
     for (uint32_t i = threadIdx.x; i < M * nv; i += 32 * kVecWarps) {
         const uint32_t m = i / nv, v = i - m * nv;
-        sa[i] = m < g.m ? *(reinterpret_cast<const uint4*>(g.a + (uint64_t)m * g.ld_a) + v) : make_uint4(0, 0, 0, 0);
+        const uint8_t* row = reinterpret_cast<const uint8_t*>(g.a) + (uint64_t)m * g.ld_a;
+        if (m >= g.m) sa[i] = make_uint4(0, 0, 0, 0);
+        else if (AT == ROWS_WHOLE) sa[i] = reinterpret_cast<const uint4*>(row)[v];
+        else sa[i] = row_vec<AT, false>(row, v, g.k);
     }
-    const uint4* w[R];                               // rows past the last channel read the last one's again
+    const uint8_t* w[R];                             // rows past the last channel read the last one's again
 #pragma unroll
-    for (uint32_t r = 0; r < R; r++) w[r] = reinterpret_cast<const uint4*>(g.w + (uint64_t)min(n0 + r, g.n - 1) * g.ld_w);
+    for (uint32_t r = 0; r < R; r++) w[r] = reinterpret_cast<const uint8_t*>(g.w) + (uint64_t)min(n0 + r, g.n - 1) * g.ld_w;
     constexpr uint32_t U = 4;                        // vectors of a row in flight in a lane
     uint4 x[U][R];
     auto load = [&](uint32_t v0) {
 #pragma unroll
         for (uint32_t u = 0; u < U; u++)
 #pragma unroll
-            for (uint32_t r = 0; r < R; r++) {
-                const uint32_t v = v0 + u * 32 + lane;
-                x[u][r] = v < nv ? __ldcs(w[r] + v) : make_uint4(0, 0, 0, 0);
-            }
+            for (uint32_t r = 0; r < R; r++) x[u][r] = row_vec<AT, true>(w[r], v0 + u * 32 + lane, g.k);
     };
     load(0);
     __syncthreads();
@@ -180,27 +218,33 @@ __global__ void __launch_bounds__(32 * kVecWarps) gemv_i8_kernel(const GemmI8Arg
     }
 }
 
-template <typename T, uint32_t M, uint32_t R>
+template <typename T, uint32_t M, uint32_t R, uint32_t AT>
 bool launch_vec(const GemmI8Args& g, cudaStream_t st) {
     const uint32_t per = kVecWarps * R;
-    return LM_CUDA(launch_k(gemv_i8_kernel<T, M, R>, dim3((g.n + per - 1) / per), dim3(32 * kVecWarps), (size_t)M * g.k, st, g));
+    return LM_CUDA(launch_k(gemv_i8_kernel<T, M, R, AT>, dim3((g.n + per - 1) / per), dim3(32 * kVecWarps),
+                            (size_t)M * ((g.k + 15) / 16 * 16), st, g));
 }
 // Two channels a warp where there are enough for every SM, else one (one token
-// x 5632 x 2048: 2.9 us with one, 3.3 with two; 22016 x 4096: 16.1, 15.5).
-template <typename T, uint32_t M>
+// x 5632 x 2048: 2.9 us with one, 3.3 with two; 22016 x 4096: 16.1, 15.6).
+template <typename T, uint32_t M, uint32_t AT>
 bool launch_vec(const GemmI8Args& g, cudaStream_t st) {
-    return M == 8 || g.n > 8192 ? launch_vec<T, M, 2>(g, st) : launch_vec<T, M, 1>(g, st);
+    return M == 8 || g.n > 8192 ? launch_vec<T, M, 2, AT>(g, st) : launch_vec<T, M, 1, AT>(g, st);
+}
+template <typename T, uint32_t AT>
+bool launch_vec(const GemmI8Args& g, cudaStream_t st) {
+    return g.m == 1 ? launch_vec<T, 1, AT>(g, st) : g.m == 2 ? launch_vec<T, 2, AT>(g, st)
+         : g.m <= 4 ? launch_vec<T, 4, AT>(g, st) : launch_vec<T, 8, AT>(g, st);
+}
+// Whether up to 8 tokens' rows fit its shared memory.
+bool vec_fits(const GemmI8Args& g) {
+    const uint32_t M = g.m <= 2 ? g.m : g.m <= 4 ? 4 : 8;
+    return g.m <= 8 && (uint64_t)M * ((g.k + 15) / 16 * 16) <= kVecSmem;
 }
 // Whether the vectors' kernel is the fastest: up to two tokens always (one token x
-// 4096 x 4096: 4.7 us against the tensor cores' 6.2; 32000 x 2048 10.9, 12.8), more
+// 4096 x 4096: 4.0 us against the tensor cores' 6.2; 32000 x 2048 10.8, 12.8), more
 // while their rows are short (four x 4096 x 4096 5.9 against 6.4, x 11008 16.3
 // against 10.8; eight x 2560 x 2048 3.4 against 4.5, 12288 x 4096 15.5 against 12.5).
-bool vec_wins(const GemmI8Args& g) {
-    if (g.k % 16 != 0 || g.m > 8) return false;
-    const uint32_t M = g.m <= 2 ? g.m : g.m <= 4 ? 4 : 8;
-    if ((uint64_t)M * g.k > kVecSmem) return false;
-    return M <= 2 || (g.k <= 4096 && (M == 4 || g.n <= 4096));
-}
+bool vec_wins(const GemmI8Args& g) { return vec_fits(g) && (g.m <= 2 || (g.k <= 4096 && (g.m <= 4 || g.n <= 4096))); }
 
 // ---------------------------------------------------------------- tensor cores
 
@@ -1015,10 +1059,8 @@ bool tma_rows(const GemmI8Args& g) {
 // all tiles, and at most 24 %.
 template <typename T>
 bool launch(const GemmI8Args& g, cudaStream_t st) {
-    if (!tma_rows(g)) return launch_any<T>(g, st);
-    if (vec_wins(g))
-        return g.m == 1 ? launch_vec<T, 1>(g, st) : g.m == 2 ? launch_vec<T, 2>(g, st)
-             : g.m <= 4 ? launch_vec<T, 4>(g, st) : launch_vec<T, 8>(g, st);
+    if (!tma_rows(g)) return vec_fits(g) ? launch_vec<T, ROWS_ANY>(g, st) : launch_any<T>(g, st);
+    if (vec_wins(g)) return g.k % 16 == 0 ? launch_vec<T, ROWS_WHOLE>(g, st) : launch_vec<T, ROWS_TAIL>(g, st);
     const uint64_t tn = (g.n + 127) / 128, sms = i8_sms();
     const uint32_t nkb = (g.k + kSlab - 1) / kSlab;
     const uint64_t wide = 6 * sms / 5, most = nkb < 30 ? wide : 3 * sms / 5;

@@ -140,6 +140,22 @@ def test_norm_sum_in_place(gpu, type, rows, cols, over):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("type", [0, 1, 30])
+@pytest.mark.parametrize("cols", [64, 100, 4096])
+def test_norm_sum_without_a_residual_and_of_a_row_with_itself(gpu, type, cols):
+    g = _gen(cols)
+    x = Rows(40, cols, DT[type], fill=_rand(g, 40, cols))
+    w = torch.ones(cols, device="cuda")
+    q, scale = Rows(40, cols, torch.int8, (-cols) % 16), torch.empty(40, device="cuda")
+    out = Rows(40, cols, DT[type])
+    _ok(gpu, _norm(gpu, type, x, None, out, w, 1e-5, 40, cols, q, scale))
+    assert torch.equal(out.t, x.t)
+    _ok(gpu, _norm(gpu, type, x, x, out, w, 1e-5, 40, cols, q, scale))
+    assert torch.equal(out.t, x.t + x.t)           # doubling is exact
+    h = 2 * x.t.double()
+    _check_int8(q.t, scale, h / (h.square().mean(1, True) + float(np.float32(1e-5))).sqrt(), _norm_r(cols))
+
+
 @pytest.mark.parametrize("cols", [5, 896, 2048, 11008, 40000])
 def test_norm_rows_of_zeros_and_of_what_is_not_finite(gpu, cols):
     x = torch.ones(6, cols, device="cuda")
@@ -390,6 +406,14 @@ def test_gemm_pitches_and_alignments(gpu, m, n, k, type, layout):
         if layout.get(key, 0) % 16 == 0 and key in layout and layout[key]:
             layout[key] += (-k) % 16
     _run_gemm(gpu, m, n, k, type, True, **layout)
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 8, 9])
+@pytest.mark.parametrize("n,k", [(1, 1), (9, 15), (77, 16), (130, 17), (9001, 35), (40, 1000), (33, 2047), (200, 4095), (3, 5001)])
+@pytest.mark.parametrize("layout", [dict(), dict(pad_a=0, pad_w=0), dict(pad_a=1, pad_w=2, shift_a=3, shift_w=1),
+                                    dict(shift_w=2, pad_w=4), dict(pad_a=13, pad_w=29, shift_w=5)])
+def test_gemm_few_tokens_at_any_address(gpu, m, n, k, layout):
+    _run_gemm(gpu, m, n, k, 0, True, **layout)
 
 
 @pytest.mark.parametrize("m,n", [(1, 40), (20, 40), (130, 300)])
