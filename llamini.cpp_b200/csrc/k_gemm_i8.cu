@@ -34,25 +34,51 @@ struct GemmI8Args {
 // that an output is the same whichever kernel and tile it comes from.
 __device__ __forceinline__ float scaled(int sum, float as, float ws) { return __fmul_rn(__fmul_rn((float)sum, as), ws); }
 
-// Rows of any pitch and alignment: 64 x 64 outputs a CTA, 64 columns of both
-// operands at a time in shared memory as words of four, dp4a on 4 x 4 outputs
-// a thread. For more than 8 tokens where TMA cannot read the rows; bound by dp4a
-// and byte loads (4096 x 4096 x 11008: 6.5 ms, 57 TOP/s).
-constexpr uint32_t kST = 64, kSW = kST / 4, kSPad = kSW + 1;
+// Rows of any pitch and alignment: 64 x 64 outputs a CTA, 64 columns of both operands
+// at a time through registers into shared memory, mma.sync on them. For more than 8
+// tokens where TMA cannot read the rows. Bound by the trip to memory of each step when
+// there are few tiles (32 tokens x 4096 x 4095: 101 us) and by the words' assembly else
+// (4096 x 4096 x 4095: 1.15 ms, 119 TOP/s). Steps of 128 and 256 columns took 102 and
+// 107 us there, and 1.90 and 2.46 ms here: their registers cost resident CTAs.
+constexpr uint32_t kST = 64, kSK = 64, kSW = kSK / 4, kSPad = kSW + 4, kSN = kST * kSW / 256;
 
-__device__ __forceinline__ void load_words(uint32_t (*dst)[kSPad], const int8_t* src, uint64_t ld, uint32_t r0,
-                                           uint32_t rows, uint32_t k0, uint32_t k) {
-    for (uint32_t i = threadIdx.x; i < kST * kSW; i += 256) {
-        const uint32_t r = i / kSW, c = i % kSW;
-        uint32_t v = 0;
-        if (r0 + r < rows) {
-            const uint8_t* p = reinterpret_cast<const uint8_t*>(src) + (uint64_t)(r0 + r) * ld;
+// The words of this thread of 64 rows x kSK columns from row r0, column k0 on;
+// zeros past the matrix. A word at any address comes from the two aligned words
+// around it, each of which holds a byte of the row.
+__device__ __forceinline__ void fetch_words(uint32_t* v, const int8_t* src, uint64_t ld, uint32_t r0, uint32_t rows, uint32_t k0,
+                                            uint32_t k) {
+#pragma unroll
+    for (uint32_t j = 0; j < kSN; j++) {
+        const uint32_t i = threadIdx.x + 256 * j, r = i / kSW, c = k0 + 4 * (i % kSW);
+        v[j] = 0;
+        if (r0 + r >= rows) continue;
+        const uint8_t* p = reinterpret_cast<const uint8_t*>(src) + (uint64_t)(r0 + r) * ld + c;
+        if (c + 7 <= k) {
+            const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(a & ~uintptr_t(3));
+            v[j] = __funnelshift_r(w[0], w[1], (uint32_t)(a & 3u) * 8u);
+        } else {
 #pragma unroll
             for (uint32_t b = 0; b < 4; b++)
-                if (k0 + 4 * c + b < k) v |= (uint32_t)p[k0 + 4 * c + b] << (8 * b);
+                if (c + b < k) v[j] |= (uint32_t)p[b] << (8 * b);
         }
-        dst[r][c] = v;
     }
+}
+__device__ __forceinline__ void put_words(uint32_t (*dst)[kSPad], const uint32_t* v) {
+#pragma unroll
+    for (uint32_t j = 0; j < kSN; j++) {
+        const uint32_t i = threadIdx.x + 256 * j;
+        dst[i / kSW][i % kSW] = v[j];
+    }
+}
+
+// D += A B of 16 x 32 and 32 x 8 int8: lane (g = lane / 4, t = lane % 4) holds of A the
+// words t and t + 4 of rows g and g + 8, of B the words t and t + 4 of column g, of D
+// columns 2 t and 2 t + 1 of rows g and g + 8.
+__device__ __forceinline__ void mma_16832(int* d, const uint32_t* a, const uint32_t* b) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
 template <typename T>
@@ -60,40 +86,41 @@ __global__ void __launch_bounds__(256) gemm_i8_any_kernel(const GemmI8Args g) {
     __shared__ uint32_t sa[kST][kSPad], sw[kST][kSPad];
     const uint32_t nt = (g.n + kST - 1) / kST;
     const uint32_t n0 = blockIdx.x % nt * kST, m0 = blockIdx.x / nt * kST;
-    const uint32_t tx = threadIdx.x & 15u, ty = threadIdx.x >> 4;
+    const uint32_t warp = threadIdx.x >> 5, gid = (threadIdx.x & 31u) >> 2, tig = threadIdx.x & 3u;
+    const uint32_t mw = (warp & 3u) * 16, nw = (warp >> 2) * 32;      // this warp's 16 tokens x 32 channels
     int acc[4][4] = {};
-    for (uint32_t k0 = 0; k0 < g.k; k0 += kST) {
-        load_words(sa, g.a, g.ld_a, m0, g.m, k0, g.k);
-        load_words(sw, g.w, g.ld_w, n0, g.n, k0, g.k);
+    uint32_t va[kSN], vw[kSN];                       // the next columns, on their way
+    fetch_words(va, g.a, g.ld_a, m0, g.m, 0, g.k);
+    fetch_words(vw, g.w, g.ld_w, n0, g.n, 0, g.k);
+    for (uint32_t k0 = 0; k0 < g.k; k0 += kSK) {
+        put_words(sa, va);
+        put_words(sw, vw);
         __syncthreads();
+        if (k0 + kSK < g.k) {
+            fetch_words(va, g.a, g.ld_a, m0, g.m, k0 + kSK, g.k);
+            fetch_words(vw, g.w, g.ld_w, n0, g.n, k0 + kSK, g.k);
+        }
 #pragma unroll
-        for (uint32_t c = 0; c < kSW; c++) {
-            uint32_t x[4], y[4];
+        for (uint32_t c = 0; c < kSW; c += 8) {
+            uint32_t a[4] = {sa[mw + gid][c + tig], sa[mw + gid + 8][c + tig], sa[mw + gid][c + tig + 4], sa[mw + gid + 8][c + tig + 4]};
 #pragma unroll
-            for (uint32_t i = 0; i < 4; i++) {
-                x[i] = sa[ty + 16 * i][c];
-                y[i] = sw[tx + 16 * i][c];
+            for (uint32_t j = 0; j < 4; j++) {
+                uint32_t b[2] = {sw[nw + j * 8 + gid][c + tig], sw[nw + j * 8 + gid][c + tig + 4]};
+                mma_16832(acc[j], a, b);
             }
-#pragma unroll
-            for (uint32_t i = 0; i < 4; i++)
-#pragma unroll
-                for (uint32_t j = 0; j < 4; j++) acc[i][j] = __dp4a((int)x[i], (int)y[j], acc[i][j]);
         }
         __syncthreads();
     }
 #pragma unroll
-    for (uint32_t i = 0; i < 4; i++) {
-        const uint32_t m = m0 + ty + 16 * i;
-        if (m >= g.m) continue;
+    for (uint32_t j = 0; j < 4; j++)
 #pragma unroll
-        for (uint32_t j = 0; j < 4; j++) {
-            const uint32_t n = n0 + tx + 16 * j;
-            if (n >= g.n) continue;
-            float v = scaled(acc[i][j], g.as[m], g.ws[n]);
+        for (uint32_t i = 0; i < 4; i++) {
+            const uint32_t m = m0 + mw + gid + (i >> 1) * 8, n = n0 + nw + j * 8 + tig * 2 + (i & 1u);
+            if (m >= g.m || n >= g.n) continue;
+            float v = scaled(acc[j][i], g.as[m], g.ws[n]);
             if (g.bias) v = __fadd_rn(v, g.bias[n]);
             static_cast<T*>(g.out)[(uint64_t)m * g.ld_out + n] = from_f32<T>(v);
         }
-    }
 }
 
 template <typename T>
@@ -112,7 +139,7 @@ bool launch_any(const GemmI8Args& g, cudaStream_t st) {
 // M tokens' rows in shared memory. dp4a keeps up with the memory (M / 4 of them a
 // weight byte), there is nothing to set up, and no SM waits for another. One token
 // x 22016 x 4096: 15.6 us, 5.8 TB/s, 89 % of the copy bandwidth; x 2560 x 2048: 2.3 us;
-// rows at odd addresses, x 4096 x 4095: 8.2 us (the tiled kernel above: 142).
+// rows at odd addresses, x 4096 x 4095: 8.2 us (the tiled kernel above: 101 for 32 tokens, as many tiles).
 constexpr uint32_t kVecWarps = 8;
 constexpr uint32_t kVecSmem = 44 * 1024;         // most bytes of the tokens' rows
 
