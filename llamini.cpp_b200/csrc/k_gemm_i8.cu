@@ -36,10 +36,10 @@ __device__ __forceinline__ float scaled(int sum, float as, float ws) { return __
 
 // Rows of any pitch and alignment: 64 x 64 outputs a CTA, 64 columns of both operands
 // at a time through registers into shared memory, mma.sync on them. For more than 8
-// tokens where TMA cannot read the rows. Bound by the trip to memory of each step when
-// there are few tiles (32 tokens x 4096 x 4095: 101 us) and by the words' assembly else
-// (4096 x 4096 x 4095: 1.15 ms, 119 TOP/s). Steps of 128 and 256 columns took 102 and
-// 107 us there, and 1.90 and 2.46 ms here: their registers cost resident CTAs.
+// tokens where TMA cannot read the rows and there are many tiles. Bound by the trip to
+// memory of each step at few (64 tokens x 22016 x 4096: 210 us) and by the words'
+// assembly else (4096 x 4096 x 4095: 1.15 ms, 119 TOP/s). Steps of 128 and 256 columns took 254 and
+// 456 us there, and 1.90 and 2.46 ms here: their registers cost resident CTAs.
 constexpr uint32_t kST = 64, kSK = 64, kSW = kSK / 4, kSPad = kSW + 4, kSN = kST * kSW / 256;
 
 // The words of this thread of 64 rows x kSK columns from row r0, column k0 on;
@@ -134,12 +134,13 @@ bool launch_any(const GemmI8Args& g, cudaStream_t st) {
     return LM_CUDA(cudaGetLastError());
 }
 
-// One to eight tokens, the products of single-sequence decoding: each warp
+// One to eight tokens, the products of single-sequence decoding (and, of rows that TMA
+// cannot read, eight of more tokens a CTA): each warp
 // streams R channels' rows, 16 bytes a lane and up to 4 R loads in flight, against
 // M tokens' rows in shared memory. dp4a keeps up with the memory (M / 4 of them a
 // weight byte), there is nothing to set up, and no SM waits for another. One token
 // x 22016 x 4096: 15.6 us, 5.8 TB/s, 89 % of the copy bandwidth; x 2560 x 2048: 2.3 us;
-// rows at odd addresses, x 4096 x 4095: 8.2 us (the tiled kernel above: 101 for 32 tokens, as many tiles).
+// rows at odd addresses, x 4096 x 4095: 8.2 us.
 constexpr uint32_t kVecWarps = 8;
 constexpr uint32_t kVecSmem = 44 * 1024;         // most bytes of the tokens' rows
 
@@ -180,8 +181,15 @@ __device__ __forceinline__ uint4 row_vec(const uint8_t* row, uint32_t v, uint32_
 }
 
 template <typename T, uint32_t M, uint32_t R, uint32_t AT>
-__global__ void __launch_bounds__(32 * kVecWarps) gemv_i8_kernel(const GemmI8Args g) {
+__global__ void __launch_bounds__(32 * kVecWarps) gemv_i8_kernel(GemmI8Args g) {
     extern __shared__ __align__(16) uint8_t sm_raw[];
+    if (AT == ROWS_ANY && M == 8) {                  // the eight tokens of this CTA
+        const uint64_t m0 = (uint64_t)blockIdx.y * M;
+        g.a += m0 * g.ld_a;
+        g.as += m0;
+        g.out = static_cast<T*>(g.out) + m0 * g.ld_out;
+        g.m -= (uint32_t)m0;
+    }
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     const uint32_t nv = (g.k + 15) / 16;             // 16-byte vectors of a row
     const uint32_t n0 = (blockIdx.x * kVecWarps + warp) * R;
@@ -248,7 +256,7 @@ __global__ void __launch_bounds__(32 * kVecWarps) gemv_i8_kernel(const GemmI8Arg
 template <typename T, uint32_t M, uint32_t R, uint32_t AT>
 bool launch_vec(const GemmI8Args& g, cudaStream_t st) {
     const uint32_t per = kVecWarps * R;
-    return LM_CUDA(launch_k(gemv_i8_kernel<T, M, R, AT>, dim3((g.n + per - 1) / per), dim3(32 * kVecWarps),
+    return LM_CUDA(launch_k(gemv_i8_kernel<T, M, R, AT>, dim3((g.n + per - 1) / per, (g.m + M - 1) / M), dim3(32 * kVecWarps),
                             (size_t)M * ((g.k + 15) / 16 * 16), st, g));
 }
 // Two channels a warp where there are enough for every SM, else one (one token
@@ -262,16 +270,24 @@ bool launch_vec(const GemmI8Args& g, cudaStream_t st) {
     return g.m == 1 ? launch_vec<T, 1, AT>(g, st) : g.m == 2 ? launch_vec<T, 2, AT>(g, st)
          : g.m <= 4 ? launch_vec<T, 4, AT>(g, st) : launch_vec<T, 8, AT>(g, st);
 }
-// Whether up to 8 tokens' rows fit its shared memory.
+// Whether the rows of up to 8 tokens fit its shared memory.
 bool vec_fits(const GemmI8Args& g) {
     const uint32_t M = g.m <= 2 ? g.m : g.m <= 4 ? 4 : 8;
-    return g.m <= 8 && (uint64_t)M * ((g.k + 15) / 16 * 16) <= kVecSmem;
+    return (uint64_t)M * ((g.k + 15) / 16 * 16) <= kVecSmem;
+}
+// Where TMA cannot read the rows: the vectors' kernel, eight tokens a CTA, unless the
+// tiles are enough to hide each other's trips to memory (16 tokens x 4096 x 4095: 25 us
+// against the tiles' 88; 128 tokens, 128 tiles: 155, 161; 128 x 2560 x 2047, 80 tiles:
+// 55, 64; 256, 160 tiles: 107, 69; 64 x 22016 x 4096, 344 tiles: 488, 210).
+bool vec_wins_any(const GemmI8Args& g) {
+    const uint64_t tiles = (uint64_t)((g.n + kST - 1) / kST) * ((g.m + kST - 1) / kST);
+    return vec_fits(g) && (g.m <= 8 || tiles <= 128);
 }
 // Whether the vectors' kernel is the fastest: up to two tokens always (one token x
 // 4096 x 4096: 4.0 us against the tensor cores' 6.2; 32000 x 2048 10.8, 12.8), more
 // while their rows are short (four x 4096 x 4096 5.9 against 6.4, x 11008 16.3
 // against 10.8; eight x 2560 x 2048 3.4 against 4.5, 12288 x 4096 15.5 against 12.5).
-bool vec_wins(const GemmI8Args& g) { return vec_fits(g) && (g.m <= 2 || (g.k <= 4096 && (g.m <= 4 || g.n <= 4096))); }
+bool vec_wins(const GemmI8Args& g) { return g.m <= 8 && vec_fits(g) && (g.m <= 2 || (g.k <= 4096 && (g.m <= 4 || g.n <= 4096))); }
 
 // ---------------------------------------------------------------- tensor cores
 
@@ -1086,7 +1102,7 @@ bool tma_rows(const GemmI8Args& g) {
 // all tiles, and at most 24 %.
 template <typename T>
 bool launch(const GemmI8Args& g, cudaStream_t st) {
-    if (!tma_rows(g)) return vec_fits(g) ? launch_vec<T, ROWS_ANY>(g, st) : launch_any<T>(g, st);
+    if (!tma_rows(g)) return vec_wins_any(g) ? launch_vec<T, ROWS_ANY>(g, st) : launch_any<T>(g, st);
     if (vec_wins(g)) return g.k % 16 == 0 ? launch_vec<T, ROWS_WHOLE>(g, st) : launch_vec<T, ROWS_TAIL>(g, st);
     const uint64_t tn = (g.n + 127) / 128, sms = i8_sms();
     const uint32_t nkb = (g.k + kSlab - 1) / kSlab;

@@ -416,6 +416,17 @@ def test_gemm_few_tokens_at_any_address(gpu, m, n, k, layout):
     _run_gemm(gpu, m, n, k, 0, True, **layout)
 
 
+# more than eight tokens where TMA cannot read: eight a CTA while there are few tiles
+# of 64 x 64 and the rows are short, else the tiles
+@pytest.mark.parametrize("m,n,k", [(9, 77, 33), (16, 260, 1000), (17, 1, 1), (65, 500, 2047), (130, 300, 5631), (8193, 5, 3),
+                                   (9, 130, 6001), (64, 64, 5700), (70, 33, 12289), (700, 1100, 333), (130, 9001, 65),
+                                   (833, 641, 64), (1000, 600, 63)])
+@pytest.mark.parametrize("layout", [dict(pad_a=0, pad_w=0), dict(pad_a=1, pad_w=2, shift_a=3, shift_w=1), dict(shift_w=2, pad_o=5)])
+@pytest.mark.parametrize("type", [0, 30])
+def test_gemm_more_tokens_at_any_address(gpu, m, n, k, layout, type):
+    _run_gemm(gpu, m, n, k, type, True, **layout)
+
+
 @pytest.mark.parametrize("m,n", [(1, 40), (20, 40), (130, 300)])
 def test_gemm_longest_sums(gpu, m, n):
     """131071 columns of -128 x -128, the largest sum: 2147467264."""
