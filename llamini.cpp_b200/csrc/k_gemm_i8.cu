@@ -491,7 +491,6 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 2) gemm_i8_few_kernel(const
     const uint32_t m0 = tile % tiles_m * NT, n0 = tile / tiles_m * 128;
     const uint32_t nkb = (g.k + kSlab - 1) / kSlab;
     const uint32_t kb0 = (uint32_t)((uint64_t)nkb * rank / cs), kb1 = (uint32_t)((uint64_t)nkb * (rank + 1) / cs);
-    pdl_trigger();
     if (threadIdx.x == 32) {
         map_prefetch(&map_w);
         map_prefetch(&map_a);
@@ -514,6 +513,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 2) gemm_i8_few_kernel(const
     __syncthreads();
     tc_after();
     const uint32_t tmem = S.tmem;
+    pdl_trigger();                                   // not before: a dependent's CTA could take the tensor memory first
     pdl_wait();
 
     if (warp == F::kEpi) {
@@ -725,7 +725,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
     const uint32_t rank = cluster_rank();
     const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const uint32_t nkb = (g.k + kSlab - 1) / kSlab;
-    pdl_trigger();
     if (threadIdx.x == 32) {
         map_prefetch(&map_w);
         map_prefetch(&map_a);
@@ -753,6 +752,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
     cluster_sync();                                  // both CTAs' barriers exist
     tc_after();
     const uint32_t tmem = S.tmem;
+    pdl_trigger();                                   // not before: a dependent's CTA could take the tensor memory first
     pdl_wait();
 
     if (warp == M::kEpi) {

@@ -2,9 +2,10 @@
 // an RMS norm with the residual's addition, and from a gated activation. They
 // feed the int8 matrix product in k_gemm_i8.cu.
 //
-// Each operator is two passes over a row: the largest magnitude (and for the
-// norm the sum of squares), then the rounding to int8 (i8.cuh). Sums, scales
-// and every value before the rounding are f32.
+// Each operator passes over a row's values twice: for the largest magnitude (and in
+// the norm the sum of squares), then for the rounding to int8 (i8.cuh). A row that
+// fits a CTA's registers is read once and kept there in between. Sums, scales and
+// every value before the rounding are f32.
 #include "i8.cuh"
 #include "pdl.cuh"
 
@@ -662,7 +663,7 @@ uint32_t rows_vectors(bool norm, uint32_t rows, uint32_t nv) {
     if (!norm && rows < 1024 && nv <= 2048) return 2;
     if (nv <= 1536) return 3;
     if (nv <= 2048) return 4;
-    return nv <= 3072 ? 6 : nv <= 4096 ? 8 : 0;
+    return nv <= 6 * 512 ? 6 : nv <= 8 * 512 ? 8 : 0;
 }
 
 // Calls LAUNCH for the shape that fits rows of `cols` elements; falls through

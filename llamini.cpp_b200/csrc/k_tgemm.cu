@@ -581,7 +581,6 @@ __device__ __forceinline__ TTile tg_tile(const TGemmArgs& a, uint32_t t) {
 __global__ void __launch_bounds__(kTThreads, 1) tgemm_kernel(const __grid_constant__ TGemmArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ TShared S;
-    pdl_trigger();
     const uint32_t NS = a.stages, NP = a.NP;
     const uint32_t ntiles = a.rblocks * a.ksplit;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
@@ -621,6 +620,7 @@ __global__ void __launch_bounds__(kTThreads, 1) tgemm_kernel(const __grid_consta
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = S.tmem;
+    pdl_trigger();                                  // not before: a dependent's CTA could take the tensor memory first
 
     if (warp == kTWarpRaw) {
         // ------------------------------------------------ raw weight bytes
