@@ -327,6 +327,14 @@ __device__ __forceinline__ void bar_drain(uint64_t* bar, uint32_t parity) {
     while (!bar_try(smem_u32(bar), parity) && now_ns() - t0 < kWaitNs) {
     }
 }
+// Behind a producer's last copy: waits for the MMAs' arrivals on `empty` for the last
+// of its `issued` stages. A CTA whose shared memory may still be arrived on must not
+// end; an arrival for a later phase is not a proof of one for an earlier.
+template <uint32_t STAGES>
+__device__ __forceinline__ void producer_tail(uint64_t* empty, uint32_t issued, volatile uint32_t* abort) {
+    for (uint32_t j = issued > STAGES ? issued - STAGES : 0; j < issued; j++)
+        if (!bar_wait(&empty[j % STAGES], (j / STAGES) & 1u, abort)) break;
+}
 __device__ __forceinline__ void map_prefetch(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
@@ -534,6 +542,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 2) gemm_i8_few_kernel(const
         if (i < kb1 - kb0 && lane == 0)              // aborted: let the copies land first
             for (uint32_t j = i > F::kStages ? i - F::kStages : 0; j < i; j++)
                 bar_drain(&S.full[j % F::kStages], (j / F::kStages) & 1u);
+        producer_tail<F::kStages>(S.empty, i, &S.abort);
     } else if (warp == F::kEpi + 1) {
         uint32_t s = 0, use = 0;
         for (uint32_t kb = kb0; kb < kb1; kb++) {
@@ -782,6 +791,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
         if (!ok && rank == 0 && lane == 0)           // aborted: let the copies land first
             for (uint32_t j = i > M::kStages ? i - M::kStages : 0; j < i; j++)
                 bar_drain(&S.full[j % M::kStages], (j / M::kStages) & 1u);
+        producer_tail<M::kStages>(S.empty, i, &S.abort);
     } else if (warp == M::kEpi + 1) {
         if (rank == 0) {
             uint32_t s = 0, use = 0, acc = 0;
@@ -813,7 +823,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
                 acc++;
             }
             if (elect_one()) mma_commit_pair(&S.done);
+            __syncwarp();
         }
+        bar_drain(&S.done, 0);                       // the commit arrives at both CTAs, behind the last MMA
     } else {
         constexpr uint32_t kCw = 128 / sizeof(T);    // channels of a staged chunk
         float* const sw = reinterpret_cast<float*>(sm + M::kStage * M::kStages + M::kEpi * M::kOut);
@@ -943,10 +955,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
         }
         if (TMA_OUT && lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
     }
+    // no MMA of the pair runs and no arrival is on its way: accf was waited for by the
+    // epilogue, empty by the producer, done by the MMA warp, and acce's arrivals come
+    // before the barrier's own
     __syncwarp();
-    if (S.abort && threadIdx.x == 0) bar_drain(&S.done, 0);
     __syncthreads();
-    cluster_sync();                                  // no arrival or MMA of the pair is on its way
+    cluster_sync();
     if (warp == M::kEpi + 1) {
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "n"(512) : "memory");

@@ -1,0 +1,73 @@
+"""The int8 operators where they could go wrong: ends of kernels, long walks,
+lengths at the edge of a launch's limits and values at the edge of a type's range.
+Definitions and tolerances as in test_gpu_i8.py."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import test_gpu_i8 as base  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+DT, F24, Rows = base.DT, base.F24, base.Rows
+
+
+def _product(gpu, m, n, k, type, seed):
+    """A product's arguments with its output; call() runs it on a stream."""
+    g = base._gen(seed)
+    a = Rows(m, k, torch.int8, (-k) % 16, 0, base._ints(g, m, k))
+    w = Rows(n, k, torch.int8, (-k) % 16, 0, base._ints(g, n, k))
+    sa = torch.rand(m, generator=g, device="cuda") * 0.01 + 0.001
+    sw = torch.rand(n, generator=g, device="cuda") * 0.001 + 0.0001
+    b = base._rand(g, n)
+
+    def call(out, stream):
+        return gpu.lib().llamini_gemm_i8_device(a.ptr, a.ld, sa.data_ptr(), m, w.ptr, w.ld, sw.data_ptr(), n, k, b.data_ptr(),
+                                                type, out.ptr, out.ld, stream)
+    return a, w, sa, sw, b, call
+
+
+# several tiles a pair of CTAs and several slabs of columns a tile, so that stages and
+# accumulators wrap from tile to tile; with and without halved last tiles; 16-byte and
+# odd output pitches
+@pytest.mark.parametrize("m,n,k,pad", [(2048, 4232, 2000, 8), (4096, 2568, 700, 0), (1000, 8000, 1152, 0), (2300, 2570, 900, 5),
+                                       (300, 32001, 640, 0)])
+@pytest.mark.parametrize("type", [0, 30])
+def test_products_of_several_tiles_a_pair(gpu, m, n, k, pad, type):
+    a, w, sa, sw, b, call = _product(gpu, m, n, k, type, m + n)
+    out = Rows(m, n, DT[type], pad)
+    base._ok(gpu, call(out, base._stream()))
+    torch.cuda.synchronize()
+    base._check_gemm(out.t, type, a.t, sa, w.t, sw, b)
+    assert out.untouched_around()
+
+
+def test_products_of_every_kernel_behind_one_another(gpu):
+    """CTAs of one product take the shared memory that those of another have just
+    left, on two streams: the same bits each time, so that nothing of a kernel that has
+    ended arrives in the next one's barriers or stages."""
+    shapes = [(600, 2304, 300), (32, 2048, 2048), (1024, 1024, 130), (3, 1000, 512), (2048, 4226, 260), (100, 896, 896)]
+    jobs = [_product(gpu, m, n, k, 30, i) + (m, n) for i, (m, n, k) in enumerate(shapes)]
+    want = []
+    for a, w, sa, sw, b, call, m, n in jobs:
+        out = Rows(m, n, torch.bfloat16)
+        base._ok(gpu, call(out, base._stream()))
+        torch.cuda.synchronize()
+        base._check_gemm(out.t, 30, a.t, sa, w.t, sw, b)
+        want.append(out.t.clone())
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[[Rows(j[6], j[7], torch.bfloat16) for j in jobs] for _ in range(8)] for _ in streams]
+    torch.cuda.synchronize()
+    for r in range(8):
+        for s, st in enumerate(streams):
+            for i in range(len(jobs)):
+                i = (i + 2 * s) % len(jobs)
+                base._ok(gpu, jobs[i][5](outs[s][r][i], st.cuda_stream))
+    torch.cuda.synchronize()
+    for per in outs:
+        for row in per:
+            for o, x in zip(row, want):
+                assert torch.equal(o.t, x)
