@@ -831,6 +831,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
         float* const sw = reinterpret_cast<float*>(sm + M::kStage * M::kStages + M::kEpi * M::kOut);
         float* const sb = sw + 256;
         uint8_t* const out = sm + M::kStage * M::kStages + warp * M::kOut;
+        // A bulk store writes whole 16-byte units and fills what lies behind the matrix's
+        // last channel with zeros: a row that ends inside a unit gets its last chunk
+        // from registers, as every chunk does where the pitch is not whole units.
+        const bool ragged = g.n * (uint32_t)sizeof(T) % 16 != 0;
         uint32_t acc = 0;
         bool bad = false;
         // the scales of a tile are loaded while the tile before is finished
@@ -920,7 +924,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
 #pragma unroll
                     for (uint32_t u = 0; u < 8; u++)
                         *reinterpret_cast<uint4*>(out + lane * 128 + ((u ^ (lane & 7u)) << 4)) = p[u];
-                    if (TMA_OUT) {
+                    if (TMA_OUT && !(ragged && n + kCw > g.n)) {
                         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                         __syncwarp();
                         if (lane == 0) {

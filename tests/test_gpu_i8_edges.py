@@ -71,3 +71,18 @@ def test_products_of_every_kernel_behind_one_another(gpu):
         for row in per:
             for o, x in zip(row, want):
                 assert torch.equal(o.t, x)
+
+
+@pytest.mark.parametrize("type", [0, 1, 30])
+@pytest.mark.parametrize("cut", range(1, 9))
+@pytest.mark.parametrize("m,n,k", [(513, 2600, 260), (1024, 4224, 130)])
+def test_product_leaves_the_end_of_a_unit_alone(gpu, m, n, k, cut, type):
+    """Rows in pitches of whole 16-byte units that end inside a unit: what lies
+    behind a row's last channel stays as it was."""
+    n -= cut
+    a, w, sa, sw, b, call = _product(gpu, m, n, k, type, cut)
+    out = Rows(m, n, DT[type], cut)
+    base._ok(gpu, call(out, base._stream()))
+    torch.cuda.synchronize()
+    base._check_gemm(out.t, type, a.t, sa, w.t, sw, b)
+    assert out.untouched_around()
