@@ -306,22 +306,26 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     return done != 0;
 }
 // Waits at most 2 s for the phase of `bar` with this parity; false when the
-// wait ran out, here or in another role of the CTA (*abort).
+// wait ran out, here or in another role of the CTA (*abort). Called by whole warps,
+// and the answer is the warp's: lanes that saw the barrier, the flag or the clock at
+// different moments vote, so that all of them go on to the same warp-wide instructions.
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort) {
     const uint32_t b = smem_u32(bar);
-    if (bar_try(b, parity)) return true;
+    if (__all_sync(0xffffffffu, bar_try(b, parity))) return true;
     const uint64_t t0 = now_ns();
     for (;;) {
-        if (bar_try(b, parity)) return true;
-        if (*abort) return false;
-        if (now_ns() - t0 > kWaitNs) {
+        if (__all_sync(0xffffffffu, bar_try(b, parity))) return true;
+        const bool out = now_ns() - t0 > kWaitNs;
+        if (__any_sync(0xffffffffu, out)) {
             *abort = 1u;
-            atomicOr(&g_i8_err, 1u);
+            if (out) atomicOr(&g_i8_err, 1u);
             return false;
         }
+        if (__any_sync(0xffffffffu, *abort)) return false;
     }
 }
-// A wait of at most 2 s that an abort does not end: for work already started.
+// A wait of at most 2 s that an abort does not end: for work already started. (Every
+// caller joins its lanes behind it.)
 __device__ __forceinline__ void bar_drain(uint64_t* bar, uint32_t parity) {
     const uint64_t t0 = now_ns();
     while (!bar_try(smem_u32(bar), parity) && now_ns() - t0 < kWaitNs) {
@@ -867,7 +871,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
             load_scales(t + pairs);
             asm volatile("bar.sync 1, 128;\n" ::: "memory");
             bad |= !bar_wait(&S.accf[buf], (acc / 2) & 1u, &S.abort);
-            bad = __any_sync(0xffffffffu, bad);
             tc_after();
             // 32 channels at a time, the next 32 on their way from tensor memory
             int v[2][32];

@@ -86,3 +86,26 @@ def test_product_leaves_the_end_of_a_unit_alone(gpu, m, n, k, cut, type):
     torch.cuda.synchronize()
     base._check_gemm(out.t, type, a.t, sa, w.t, sw, b)
     assert out.untouched_around()
+
+
+@pytest.mark.parametrize("m,n,k", [(64, 5632, 11008), (16, 2560, 8192), (1024, 4096, 4096)])
+def test_products_while_copies_hold_them_up(gpu, m, n, k):
+    """Stages arrive late and unevenly beside a stream of copies, so that the waits
+    inside the kernels really wait: the same bits as in a quiet run, and none runs out."""
+    a, w, sa, sw, b, call = _product(gpu, m, n, k, 30, m)
+    quiet = Rows(m, n, torch.bfloat16)
+    base._ok(gpu, call(quiet, base._stream()))
+    torch.cuda.synchronize()
+    base._check_gemm(quiet.t, 30, a.t, sa, w.t, sw, b)
+    src, dst = (torch.zeros(256 << 20, dtype=torch.uint8, device="cuda") for _ in range(2))
+    copies, products = torch.cuda.Stream(), torch.cuda.Stream()
+    outs = [Rows(m, n, torch.bfloat16) for _ in range(10)]
+    torch.cuda.synchronize()
+    for out in outs:
+        with torch.cuda.stream(copies):
+            dst.copy_(src, non_blocking=True)
+        base._ok(gpu, call(out, products.cuda_stream))
+    torch.cuda.synchronize()
+    for out in outs:
+        assert torch.equal(out.t, quiet.t)
+    base._ok(gpu, gpu.lib().llamini_i8_status(base._stream()))
