@@ -181,6 +181,7 @@ SIGNATURES = {
     "llamini_rms_norm_i8_device": (C.c_int, [u32, P, u64, P, u64, P, u64, P, f32, u32, u32, P, u64, P, P]),
     "llamini_glu_i8_device": (C.c_int, [u32, P, u64, P, u64, u32, u32, u32, P, u64, P, P]),
     "llamini_gemm_i8_device": (C.c_int, [P, u64, P, u32, P, u64, P, u32, u32, P, u32, P, u64, P]),
+    "llamini_set_i8_wait_ns": (C.c_int, [u64]),
     "llamini_i8_status": (C.c_int, [P]),
     "llamini_session_trace": (C.c_int, [P, C.c_int]),
     "llamini_session_trace_read": (C.c_int, [P, P]),

@@ -27,6 +27,7 @@ struct GemmI8Args {
     const float* bias;         // may be null
     void* out;
     uint64_t ld_a, ld_w, ld_out;
+    uint64_t wait_ns;          // bound of a wait inside the tensor-core kernels
     uint32_t m, n, k;
 };
 
@@ -292,7 +293,7 @@ bool vec_wins(const GemmI8Args& g) { return g.m <= 8 && vec_fits(g) && (g.m <= 2
 // ---------------------------------------------------------------- tensor cores
 
 constexpr uint32_t kSlab = 128;                  // columns (bytes) of both operands in a stage
-constexpr uint64_t kWaitNs = 2000000000ull;      // 2 s
+constexpr uint64_t kWaitNs = 2000000000ull;      // 2 s, unless llamini_set_i8_wait_ns says otherwise
 
 __device__ __forceinline__ uint64_t now_ns() {
     uint64_t t;
@@ -305,23 +306,36 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
                  " selp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(bar), "r"(parity), "n"(1000000) : "memory");
     return done != 0;
 }
-// Waits at most 2 s for the phase of `bar` with this parity; false when the
-// wait ran out, here or in another role of the CTA (*abort). Called by whole warps,
-// and the answer is the warp's: lanes that saw the barrier, the flag or the clock at
-// different moments vote, so that all of them go on to the same warp-wide instructions.
-__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort) {
+// How long a wait may take (0: it gives up without looking) and whom it tells when it
+// runs out: the CTA's flag, and the flag of the pair's other CTA (an address in the
+// cluster's shared memory, or kNoPeer).
+constexpr uint32_t kNoPeer = 0xffffffffu;
+struct Patience {
+    uint64_t ns;
+    volatile uint32_t* abort;
+    uint32_t peer;
+};
+__device__ __forceinline__ void cluster_st(uint32_t a, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(a), "r"(v) : "memory");
+}
+// Waits for the phase of `bar` with this parity; false when the wait ran out, here
+// or in another role (*abort). Called by whole warps, and the answer is the warp's:
+// lanes that saw the barrier, the flag or the clock at different moments vote, so that
+// all of them go on to the same warp-wide instructions.
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, const Patience& p) {
     const uint32_t b = smem_u32(bar);
-    if (__all_sync(0xffffffffu, bar_try(b, parity))) return true;
+    if (p.ns && __all_sync(0xffffffffu, bar_try(b, parity))) return true;
     const uint64_t t0 = now_ns();
     for (;;) {
-        if (__all_sync(0xffffffffu, bar_try(b, parity))) return true;
-        const bool out = now_ns() - t0 > kWaitNs;
+        if (p.ns && __all_sync(0xffffffffu, bar_try(b, parity))) return true;
+        const bool out = now_ns() - t0 >= p.ns;
         if (__any_sync(0xffffffffu, out)) {
-            *abort = 1u;
+            *p.abort = 1u;
+            if (p.peer != kNoPeer) cluster_st(p.peer, 1u);
             if (out) atomicOr(&g_i8_err, 1u);
             return false;
         }
-        if (__any_sync(0xffffffffu, *abort)) return false;
+        if (__any_sync(0xffffffffu, *p.abort)) return false;
     }
 }
 // A wait of at most 2 s that an abort does not end: for work already started. (Every
@@ -335,9 +349,9 @@ __device__ __forceinline__ void bar_drain(uint64_t* bar, uint32_t parity) {
 // of its `issued` stages. A CTA whose shared memory may still be arrived on must not
 // end; an arrival for a later phase is not a proof of one for an earlier.
 template <uint32_t STAGES>
-__device__ __forceinline__ void producer_tail(uint64_t* empty, uint32_t issued, volatile uint32_t* abort) {
+__device__ __forceinline__ void producer_tail(uint64_t* empty, uint32_t issued, const Patience& p) {
     for (uint32_t j = issued > STAGES ? issued - STAGES : 0; j < issued; j++)
-        if (!bar_wait(&empty[j % STAGES], (j / STAGES) & 1u, abort)) break;
+        if (!bar_wait(&empty[j % STAGES], (j / STAGES) & 1u, p)) break;
 }
 __device__ __forceinline__ void map_prefetch(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
@@ -407,9 +421,6 @@ __device__ __forceinline__ int4 cluster_ld4(uint32_t a) {
     int4 v;
     asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
     return v;
-}
-__device__ __forceinline__ void cluster_st(uint32_t a, uint32_t v) {
-    asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(a), "r"(v) : "memory");
 }
 
 // This CTA's share of a tile's tokens (NT rows of 128 sums in every CTA of the
@@ -525,13 +536,15 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 2) gemm_i8_few_kernel(const
     __syncthreads();
     tc_after();
     const uint32_t tmem = S.tmem;
+    const Patience wait = {g.wait_ns, &S.abort, kNoPeer};
+    uint32_t issued = 0;                             // stages whose copies this CTA has started
     pdl_trigger();                                   // not before: a dependent's CTA could take the tensor memory first
     pdl_wait();
 
     if (warp == F::kEpi) {
-        uint32_t i = 0, s = 0, use = 0;              // stages so far; i = use * kStages + s
-        for (uint32_t kb = kb0; kb < kb1; kb++, i++) {
-            if (use && !bar_wait(&S.empty[s], (use - 1) & 1u, &S.abort)) break;
+        uint32_t s = 0, use = 0;                     // issued = use * kStages + s
+        for (uint32_t kb = kb0; kb < kb1; kb++, issued++) {
+            if (use && !bar_wait(&S.empty[s], (use - 1) & 1u, wait)) break;
             if (elect_one()) {
                 mbar_expect_tx(&S.full[s], F::kStage);
                 tile_load(base + s * F::kStage, &map_w, kb * kSlab, n0, &S.full[s]);
@@ -543,14 +556,11 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 2) gemm_i8_few_kernel(const
                 use++;
             }
         }
-        if (i < kb1 - kb0 && lane == 0)              // aborted: let the copies land first
-            for (uint32_t j = i > F::kStages ? i - F::kStages : 0; j < i; j++)
-                bar_drain(&S.full[j % F::kStages], (j / F::kStages) & 1u);
-        producer_tail<F::kStages>(S.empty, i, &S.abort);
+        producer_tail<F::kStages>(S.empty, issued, wait);
     } else if (warp == F::kEpi + 1) {
         uint32_t s = 0, use = 0;
         for (uint32_t kb = kb0; kb < kb1; kb++) {
-            if (!bar_wait(&S.full[s], use & 1u, &S.abort)) break;
+            if (!bar_wait(&S.full[s], use & 1u, wait)) break;
             tc_after();
             if (elect_one()) {
                 const uint32_t steps = (g.k - kb * kSlab + 31) / 32;
@@ -580,7 +590,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 2) gemm_i8_few_kernel(const
         }
         if (threadIdx.x < mt) S.as[threadIdx.x] = g.as[m0 + threadIdx.x];
         // every copy has landed and been read once the last MMA has finished
-        if (!bar_wait(&S.done, 0, &S.abort)) bar_drain(&S.done, 0);
+        if (!bar_wait(&S.done, 0, wait)) bar_drain(&S.done, 0);
         __syncwarp();
         tc_after();
         for (uint32_t c = (warp >> 2) * 16; c < mt; c += 32) {
@@ -597,9 +607,9 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 2) gemm_i8_few_kernel(const
         __syncwarp();
         cluster_sync();
     }
+    const uint32_t bad = S.abort;                    // (every role has ended)
     if (warp < F::kEpi) {
         const bool vec = (reinterpret_cast<uintptr_t>(g.out) | (g.ld_out * sizeof(T))) % (4 * sizeof(T)) == 0;
-        const uint32_t bad = S.abort;
         auto finish = [&](uint32_t t, const int4& v) {
             const float as = bad ? NAN : S.as[t];
             const int x[4] = {v.x, v.y, v.z, v.w};
@@ -628,6 +638,10 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 2) gemm_i8_few_kernel(const
     __syncwarp();
     if (cs > 1) cluster_sync();
     else __syncthreads();
+    // after a wait that ran out, copies may still be on their way into this CTA
+    if (warp == F::kEpi && bad)
+        for (uint32_t j = issued > F::kStages ? issued - F::kStages : 0; j < issued; j++)
+            bar_drain(&S.full[j % F::kStages], (j / F::kStages) & 1u);
     if (warp == F::kEpi + 1) {
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "n"(F::kCols) : "memory");
@@ -665,6 +679,7 @@ struct Many {
 struct ManyShared {
     uint64_t full[8], empty[8], accf[2], acce[2], done;
     uint32_t tmem, abort;
+    uint32_t issued[2];        // (of the first CTA) stages whose copies each CTA has started
 };
 
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t cluster_bar) {
@@ -684,6 +699,10 @@ __device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t a, uint64_t b, 
 __device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
                  ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+}
+// Takes `bytes` off what the current phase of `bar` still waits for.
+__device__ __forceinline__ void mbar_complete_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 // 32 columns of this warp's 32 tensor-memory lanes; the registers are valid
 // after tmem_wait32, which every use has to follow.
@@ -765,6 +784,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
     cluster_sync();                                  // both CTAs' barriers exist
     tc_after();
     const uint32_t tmem = S.tmem;
+    const Patience wait = {g.wait_ns, &S.abort, cluster_addr(smem_u32(&S.abort), rank ^ 1u)};
     pdl_trigger();                                   // not before: a dependent's CTA could take the tensor memory first
     pdl_wait();
 
@@ -777,7 +797,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
             const uint32_t ra = q.tm * 256 + rank * 128, rw = q.n0 + rank * (q.bn / 2);
             const bool whole = q.bn == 256;
             for (uint32_t kb = 0; kb < nkb; kb++, i++) {
-                if (use && !(ok = bar_wait(&S.empty[s], (use - 1) & 1u, &S.abort))) break;
+                if (use && !(ok = bar_wait(&S.empty[s], (use - 1) & 1u, wait))) break;
                 const uint32_t full = cluster_addr(smem_u32(&S.full[s]), 0), at = base + s * M::kStage;
                 if (elect_one()) {
                     if (rank == 0) mbar_expect_tx(&S.full[s], 2 * (M::kA + (whole ? 2 : 1) * M::kB));
@@ -792,10 +812,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
                 }
             }
         }
-        if (!ok && rank == 0 && lane == 0)           // aborted: let the copies land first
-            for (uint32_t j = i > M::kStages ? i - M::kStages : 0; j < i; j++)
-                bar_drain(&S.full[j % M::kStages], (j / M::kStages) & 1u);
-        producer_tail<M::kStages>(S.empty, i, &S.abort);
+        if (lane == 0) cluster_st(cluster_addr(smem_u32(&S.issued[rank]), 0), i);
+        producer_tail<M::kStages>(S.empty, i, wait);
     } else if (warp == M::kEpi + 1) {
         if (rank == 0) {
             uint32_t s = 0, use = 0, acc = 0;
@@ -805,9 +823,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
                 if (q.n0 >= g.n) continue;
                 const uint32_t buf = acc & 1u, d = tmem + buf * 256;
                 const uint32_t idesc = q.bn == 256 ? i8_idesc(256, 256) : i8_idesc(256, 128);
-                if (acc >= 2 && !(ok = bar_wait(&S.acce[buf], (acc / 2 - 1) & 1u, &S.abort))) break;
+                if (acc >= 2 && !(ok = bar_wait(&S.acce[buf], (acc / 2 - 1) & 1u, wait))) break;
                 for (uint32_t kb = 0; kb < nkb; kb++) {
-                    if (!(ok = bar_wait(&S.full[s], use & 1u, &S.abort))) break;
+                    if (!(ok = bar_wait(&S.full[s], use & 1u, wait))) break;
                     tc_after();
                     if (elect_one()) {
                         const uint64_t da = tile_desc(base + s * M::kStage), dw = tile_desc(base + s * M::kStage + M::kA);
@@ -870,7 +888,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
             const float as = as_next;
             load_scales(t + pairs);
             asm volatile("bar.sync 1, 128;\n" ::: "memory");
-            bad |= !bar_wait(&S.accf[buf], (acc / 2) & 1u, &S.abort);
+            bad |= !bar_wait(&S.accf[buf], (acc / 2) & 1u, wait);
             tc_after();
             // 32 channels at a time, the next 32 on their way from tensor memory
             int v[2][32];
@@ -968,6 +986,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many::kThreads, 1)
     __syncwarp();
     __syncthreads();
     cluster_sync();
+    // After a wait that ran out (both CTAs know by now) copies may still be on their way.
+    // All are counted on the first CTA's barriers, which expect both CTAs' bytes: where
+    // only one of them started a stage, the other's share is taken off (or was never
+    // asked for), and then the phase ends with the last byte that does come.
+    if (S.abort) {
+        if (rank == 0 && warp == M::kEpi) {
+            const uint32_t i0 = S.issued[0], i1 = S.issued[1], n = max(i0, i1);
+            for (uint32_t j = n > M::kStages ? n - M::kStages : 0; j < n; j++) {
+                uint64_t* const full = &S.full[j % M::kStages];
+                const uint32_t bytes = M::kA + (tile_at(pair + j / nkb * pairs, tiles).bn == 256 ? 2 : 1) * M::kB;
+                if (lane == 0 && j >= i0) mbar_expect_tx(full, bytes);
+                if (lane == 0 && j >= i1) mbar_complete_tx(full, bytes);
+                __syncwarp();
+                bar_drain(full, (j / M::kStages) & 1u);
+                __syncwarp();
+            }
+        }
+        __syncwarp();
+        cluster_sync();
+    }
     if (warp == M::kEpi + 1) {
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "n"(512) : "memory");
@@ -1139,8 +1177,21 @@ bool launch(const GemmI8Args& g, cudaStream_t st) {
     }
 }
 
+std::atomic<uint64_t> g_i8_wait_ns{kWaitNs};
+constexpr uint64_t kMaxWaitNs = 60000000000ull;  // 60 s
+
 }  // namespace
 }  // namespace lm
+
+extern "C" int llamini_set_i8_wait_ns(u64 ns) {
+    using namespace lm;
+    if (ns > kMaxWaitNs) {
+        set_error("set_i8_wait_ns: %llu ns (at most %llu)", (unsigned long long)ns, (unsigned long long)kMaxWaitNs);
+        return -1;
+    }
+    g_i8_wait_ns.store(ns, std::memory_order_relaxed);
+    return 0;
+}
 
 extern "C" int llamini_gemm_i8_device(const i8* d_a, u64 ld_a, const f32* d_a_scale, u32 rows, const i8* d_w, u64 ld_w,
                                       const f32* d_w_scale, u32 n, u32 cols, const f32* d_bias, u32 out_type,
@@ -1170,6 +1221,7 @@ extern "C" int llamini_gemm_i8_device(const i8* d_a, u64 ld_a, const f32* d_a_sc
     g.bias = d_bias; g.out = d_out;
     g.ld_a = ld_a; g.ld_w = ld_w; g.ld_out = ld_out;
     g.m = rows; g.n = n; g.k = cols;
+    g.wait_ns = g_i8_wait_ns.load(std::memory_order_relaxed);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool ok = out_type == GGML_TYPE_F32 ? launch<float>(g, st)
                   : out_type == GGML_TYPE_F16 ? launch<__half>(g, st) : launch<__nv_bfloat16>(g, st);

@@ -109,3 +109,36 @@ def test_products_while_copies_hold_them_up(gpu, m, n, k):
     for out in outs:
         assert torch.equal(out.t, quiet.t)
     base._ok(gpu, gpu.lib().llamini_i8_status(base._stream()))
+
+
+# one CTA a tile, clusters of two, four and eight CTAs a tile, pairs with fewer slabs
+# than stages, with more, and with several tiles a pair
+@pytest.mark.parametrize("m,n,k", [(16, 4000, 128), (128, 20000, 700), (64, 9000, 2000), (40, 2560, 4096), (16, 896, 4096),
+                                   (512, 2304, 300), (600, 4224, 2000), (2048, 8000, 640)])
+@pytest.mark.parametrize("type", [0, 30])
+def test_product_whose_waits_run_out(gpu, m, n, k, type):
+    """A kernel that gives up: its outputs are NaN, the status says so once, nothing
+    outside the outputs is written, and the next call finds everything in order."""
+    a, w, sa, sw, b, call = _product(gpu, m, n, k, type, n)
+    L, st = gpu.lib(), base._stream()
+    base._ok(gpu, L.llamini_i8_status(st))
+    out = Rows(m, n, DT[type], 1)
+    try:
+        base._ok(gpu, L.llamini_set_i8_wait_ns(0))
+        for _ in range(3):
+            base._ok(gpu, call(out, st))
+        base._ok(gpu, L.llamini_set_i8_wait_ns(2_000_000_000))
+        assert L.llamini_i8_status(st) == -1
+        assert "wait inside a kernel ran out" in gpu.last_error()
+        L.llamini_clear_error()
+        base._ok(gpu, L.llamini_i8_status(st))
+    finally:
+        L.llamini_set_i8_wait_ns(2_000_000_000)
+        L.llamini_i8_status(st)
+        L.llamini_clear_error()
+    assert torch.isnan(out.t).all() and out.untouched_around()
+    for _ in range(3):
+        base._ok(gpu, call(out, st))
+    torch.cuda.synchronize()
+    base._check_gemm(out.t, type, a.t, sa, w.t, sw, b)
+    base._ok(gpu, L.llamini_i8_status(st))

@@ -129,3 +129,13 @@ def test_status_without_a_device(lm):
     assert L.llamini_i8_status(None) == -1
     assert "no usable CUDA device" in lm.last_error()
     L.llamini_clear_error()
+
+
+def test_wait_bound_is_limited(lm):
+    L = lm.lib()
+    L.llamini_clear_error()
+    assert L.llamini_set_i8_wait_ns(60_000_000_001) == -1
+    assert "at most 60000000000" in lm.last_error()
+    L.llamini_clear_error()
+    assert L.llamini_set_i8_wait_ns(60_000_000_000) == 0
+    assert L.llamini_set_i8_wait_ns(2_000_000_000) == 0
