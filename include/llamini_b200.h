@@ -162,9 +162,11 @@ int llamini_gemm_i8_device(const i8* d_a, u64 ld_a, const f32* d_a_scale, u32 ro
  * to two tokens, and rows that are not in 16-byte pitches, have no waits to run out). */
 int llamini_set_i8_wait_ns(u64 ns);
 
-/* Waits for `stream`, then 0, or -1 when a bounded wait inside a product's
- * kernel has run out on the current device since the last call: the outputs it
- * was for are NaN. Not during a stream capture. */
+/* Waits for `stream`, then 0, or -1 when a bounded wait inside a product's kernel has
+ * run out on the current device, on this stream or another, since the last call for
+ * this stream (for its first: since the library was loaded). The outputs of such a
+ * product are NaN; a call for one stream takes nothing away from another's. Not during
+ * a stream capture. */
 int llamini_i8_status(void* stream);
 
 /* ---- device-resident decoding sessions (generate.c:122-167 without host

@@ -11,12 +11,17 @@
 
 #include <atomic>
 #include <cudaTypedefs.h>
+#include <map>
+#include <mutex>
 #include <type_traits>
+#include <utility>
 
 namespace lm {
 namespace {
 
-// Set by a kernel whose bounded wait ran out (the outputs of its tile are NaN).
+// Bounded waits that have run out on this device (the outputs of their tiles are NaN).
+// Only ever counted up: what is new since a stream's last look is for the host to tell,
+// so that no look takes a report away from another stream's.
 __device__ uint32_t g_i8_err;
 
 struct GemmI8Args {
@@ -332,7 +337,7 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, const P
         if (__any_sync(0xffffffffu, out)) {
             *p.abort = 1u;
             if (p.peer != kNoPeer) cluster_st(p.peer, 1u);
-            if (out) atomicOr(&g_i8_err, 1u);
+            if ((threadIdx.x & 31u) == 0) atomicAdd(&g_i8_err, 1u);
             return false;
         }
         if (__any_sync(0xffffffffu, *p.abort)) return false;
@@ -1230,16 +1235,30 @@ extern "C" int llamini_gemm_i8_device(const i8* d_a, u64 ld_a, const f32* d_a_sc
 
 extern "C" int llamini_i8_status(void* stream) {
     using namespace lm;
+    const char* who = "i8_status";
     const void* none[1] = {nullptr};
-    if (!i8_device_ptrs("i8_status", none, 1)) return -1;
+    if (!i8_device_ptrs(who, none, 1)) return -1;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    uint32_t err = 0, zero = 0;
-    if (!LM_CUDA(cudaMemcpyFromSymbolAsync(&err, g_i8_err, sizeof(err), 0, cudaMemcpyDeviceToHost, st)) ||
+    int dev = 0;
+    unsigned long long id = 0;                       // of the stream; no later one has it again
+    uint32_t count = 0;
+    if (!LM_CUDA(cudaGetDevice(&dev)) || !LM_CUDA(cudaStreamGetId(st, &id)) || !LM_CUDA(cudaStreamSynchronize(st)) ||
+        !LM_CUDA(cudaMemcpyFromSymbolAsync(&count, g_i8_err, sizeof(count), 0, cudaMemcpyDeviceToHost, st)) ||
         !LM_CUDA(cudaStreamSynchronize(st)))
         return -1;
-    if (err == 0) return 0;
+    bool same = false;
+    try {
+        static std::mutex mu;
+        static std::map<std::pair<int, unsigned long long>, uint32_t> seen;
+        std::lock_guard<std::mutex> lock(mu);
+        uint32_t& last = seen[{dev, id}];
+        same = last == count;
+        last = count;
+    } catch (...) {
+        set_error("%s: out of memory", who);
+        return -1;
+    }
+    if (same) return 0;
     set_error("gemm_i8: a wait inside a kernel ran out; the outputs it was for are NaN");
-    LM_CUDA(cudaMemcpyToSymbolAsync(g_i8_err, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, st));
-    LM_CUDA(cudaStreamSynchronize(st));
     return -1;
 }

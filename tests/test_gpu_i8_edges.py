@@ -142,3 +142,32 @@ def test_product_whose_waits_run_out(gpu, m, n, k, type):
     torch.cuda.synchronize()
     base._check_gemm(out.t, type, a.t, sa, w.t, sw, b)
     base._ok(gpu, L.llamini_i8_status(st))
+
+
+def test_status_of_one_stream_leaves_the_other_its_report(gpu):
+    """Each stream's status call reports a wait that ran out once, whichever
+    stream's product it was and whoever asked before."""
+    a, w, sa, sw, b, call = _product(gpu, 64, 2304, 2048, 0, 5)
+    L = gpu.lib()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    handles = [s.cuda_stream for s in streams] + [None]
+    out = Rows(64, 2304, torch.float32)
+    try:
+        for h in handles:
+            L.llamini_i8_status(h)                 # whatever came before this test
+            L.llamini_clear_error()
+            base._ok(gpu, L.llamini_i8_status(h))
+        torch.cuda.synchronize()
+        for ran_on in handles:
+            base._ok(gpu, L.llamini_set_i8_wait_ns(0))
+            base._ok(gpu, call(out, ran_on))
+            base._ok(gpu, L.llamini_set_i8_wait_ns(2_000_000_000))
+            torch.cuda.synchronize()
+            assert [L.llamini_i8_status(h) for h in handles] == [-1, -1, -1]
+            L.llamini_clear_error()
+            assert [L.llamini_i8_status(h) for h in handles] == [0, 0, 0]
+    finally:
+        L.llamini_set_i8_wait_ns(2_000_000_000)
+        for h in handles:
+            L.llamini_i8_status(h)
+        L.llamini_clear_error()
