@@ -1239,6 +1239,9 @@ extern "C" int llamini_i8_status(void* stream) {
     const void* none[1] = {nullptr};
     if (!i8_device_ptrs(who, none, 1)) return -1;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (!LM_CUDA(cudaStreamIsCapturing(st, &capture))) return -1;
+    if (capture != cudaStreamCaptureStatusNone) { set_error("%s: the stream is being captured", who); return -1; }
     int dev = 0;
     unsigned long long id = 0;                       // of the stream; no later one has it again
     uint32_t count = 0;

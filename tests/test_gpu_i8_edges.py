@@ -171,3 +171,22 @@ def test_status_of_one_stream_leaves_the_other_its_report(gpu):
         for h in handles:
             L.llamini_i8_status(h)
         L.llamini_clear_error()
+
+
+def test_status_of_a_stream_in_capture_is_refused(gpu):
+    """The refusal leaves the capture whole."""
+    a, w, sa, sw, b, call = _product(gpu, 64, 300, 512, 0, 6)
+    L = gpu.lib()
+    want, out = Rows(64, 300, torch.float32), Rows(64, 300, torch.float32)
+    base._ok(gpu, call(want, base._stream()))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert L.llamini_i8_status(base._stream()) == -1
+        assert "being captured" in gpu.last_error()
+        L.llamini_clear_error()
+        base._ok(gpu, call(out, base._stream()))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out.t, want.t)
+    base._ok(gpu, L.llamini_i8_status(base._stream()))
