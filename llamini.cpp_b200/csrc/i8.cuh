@@ -16,6 +16,7 @@
 #include "internal.h"
 #include "llamini_b200.h"
 
+#include <atomic>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
@@ -66,6 +67,19 @@ inline uint32_t i8_sms() {
         return (uint32_t)n;
     }();
     return sms;
+}
+
+// The kernel's limit on dynamic shared memory, raised once a device. (Unasked a CTA gets
+// 48 KB of static and dynamic shared memory together.)
+template <typename K>
+inline bool allow_smem(std::atomic<uint64_t>& done, K* kernel, size_t bytes) {
+    int dev = 0;
+    if (!LM_CUDA(cudaGetDevice(&dev))) return false;
+    const uint64_t bit = 1ull << (dev & 63);             // (a device past the 63rd sets it at each call)
+    if (dev < 64 && done.load(std::memory_order_acquire) & bit) return true;
+    if (!LM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes))) return false;
+    done.fetch_or(bit, std::memory_order_release);
+    return true;
 }
 
 inline bool i8_aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }

@@ -1072,18 +1072,6 @@ cudaError_t launch_cluster(void (*kernel)(KArgs...), uint32_t grid, uint32_t blo
     return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
-// The kernel's limit on dynamic shared memory, raised once a device.
-template <typename K>
-bool allow_smem(std::atomic<uint64_t>& done, K* kernel, size_t bytes) {
-    int dev = 0;
-    if (!LM_CUDA(cudaGetDevice(&dev))) return false;
-    const uint64_t bit = 1ull << (dev & 63);             // (a device past the 63rd sets it at each call)
-    if (dev < 64 && done.load(std::memory_order_acquire) & bit) return true;
-    if (!LM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes))) return false;
-    done.fetch_or(bit, std::memory_order_release);
-    return true;
-}
-
 template <typename T, int NT>
 bool launch_few(const GemmI8Args& g, cudaStream_t st) {
     using F = Few<NT>;

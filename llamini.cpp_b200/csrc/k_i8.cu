@@ -556,9 +556,8 @@ bool launch_weights(const WeightArgs& a, cudaStream_t st) {
         while (rows > 1 && rows * a.row_bytes > kWRow / 4) rows--;
         const uint32_t buf = ((uint32_t)(rows * a.row_bytes) + kWSlack + 15u) & ~15u, smem = 2 * buf;
         auto* kernel = U == 1 ? weights_i8_rows_kernel<T, 1> : weights_i8_rows_kernel<T, 2>;
-        if (smem > 48 * 1024 &&
-            !LM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * (kWRow + kWSlack + 16)))))
-            return false;
+        static std::atomic<uint64_t> ready[2];
+        if (!allow_smem(ready[U - 1], kernel, 2 * (kWRow + kWSlack + 16))) return false;
         // CTAs that run at once: by threads and shared memory, two by registers at 512 threads
         uint32_t occ = (200 * 1024) / (smem + 1024);
         if (occ * rows * tpr > 1024) occ = 1024 / (rows * tpr);
@@ -567,9 +566,8 @@ bool launch_weights(const WeightArgs& a, cudaStream_t st) {
         return LM_CUDA(launch_k(kernel, dim3(groups < most ? groups : most), dim3(rows * tpr), smem, st, a, tpr, buf));
     }
     const uint32_t smem = (uint32_t)(a.row_bytes < kWSeg ? a.row_bytes : kWSeg) + kWSlack;
-    if (smem > 48 * 1024 &&
-        !LM_CUDA(cudaFuncSetAttribute(weights_i8_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kWSeg + kWSlack))))
-        return false;
+    static std::atomic<uint64_t> ready{0};
+    if (!allow_smem(ready, weights_i8_kernel<T>, kWSeg + kWSlack)) return false;
     weights_i8_kernel<T><<<a.rows, kWThreads, smem, st>>>(a);
     return LM_CUDA(cudaGetLastError());
 }

@@ -3,11 +3,16 @@ lengths at the edge of a launch's limits and values at the edge of a type's rang
 Definitions and tolerances as in test_gpu_i8.py."""
 from __future__ import annotations
 
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
 
+import conftest  # noqa: E402
 import test_gpu_i8 as base  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -190,3 +195,55 @@ def test_status_of_a_stream_in_capture_is_refused(gpu):
     torch.cuda.synchronize()
     assert torch.equal(out.t, want.t)
     base._ok(gpu, L.llamini_i8_status(base._stream()))
+
+
+# ---------------------------------------------------------------- weights
+
+BLOCK = {2: (32, 18), 3: (32, 20), 6: (32, 22), 8: (32, 34), 12: (256, 144), 13: (256, 176), 14: (256, 210)}
+# the longest rows whose dynamic shared memory alone stays within a CTA's default 48 KB
+# while static and dynamic together do not, and rows on either side
+DEFAULT_SMEM, SLACK, STATIC = 48 * 1024, 64, 256
+
+
+def _edge_lengths(t):
+    be, bb = BLOCK[t]
+    last = (DEFAULT_SMEM - SLACK) // bb            # blocks of a row
+    first = (DEFAULT_SMEM - SLACK - STATIC) // bb + 1
+    return [n * be for n in sorted({first - 1, first, last, last + 1})]
+
+
+def _check_weights(gpu, orc, synth, t, rows, cols, pad=0, shift=0):
+    raw = synth.random_blocks(np.random.default_rng(t + cols), t, rows * cols)
+    w = torch.from_numpy(orc.dequant(t, raw, rows * cols).reshape(rows, cols)).cuda()
+    want_q, want_s = base._want_weights(w)
+    d = torch.empty(raw.size + shift, dtype=torch.uint8, device="cuda")
+    d[shift:].copy_(torch.from_numpy(raw))
+    q = Rows(rows, cols, torch.int8, pad)
+    scale = torch.full((rows + 2,), 7.0, device="cuda")
+    base._ok(gpu, base._weights_call(gpu, t, d.data_ptr() + shift, rows, cols, q, scale))
+    torch.cuda.synchronize()
+    assert torch.equal(scale[:rows], want_s) and torch.all(scale[rows:] == 7), (t, cols)
+    assert torch.equal(q.t, want_q) and q.untouched_around(), (t, cols)
+
+
+def weights_at_the_edge_of_shared_memory(gpu, orc, synth):
+    for t in BLOCK:
+        for cols in _edge_lengths(t):              # rising: no call finds a limit raised by a longer one
+            _check_weights(gpu, orc, synth, t, 2, cols)
+
+
+def test_weights_at_the_edge_of_shared_memory(gpu, orc):
+    """Rows that need a little more shared memory than a launch gets unasked, in a
+    process whose first calls they are."""
+    code = ("import sys; sys.path[:0] = %r\n"
+            "import conftest, oracle, tiny, test_gpu_i8_edges as t\n"
+            "t.weights_at_the_edge_of_shared_memory(conftest._load_pkg(), oracle, tiny.synthetic())\n"
+            % [os.path.dirname(__file__), conftest.GOLDEN, os.path.join(conftest.ROOT, "oracle")])
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("t", sorted(BLOCK))
+@pytest.mark.parametrize("cols,pad,shift", [(98304, 0, 0), (130816, 3, 2), (106752, 16, 14)])
+def test_weights_in_several_segments(gpu, orc, synth, t, cols, pad, shift):
+    _check_weights(gpu, orc, synth, t, 3, cols, pad, shift)
