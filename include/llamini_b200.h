@@ -142,7 +142,8 @@ int llamini_rms_norm_i8_device(u32 type, const void* d_x, u64 ld_x, const void* 
 
 /* y = act(gate) * up, or act(gate) when d_up is NULL (ffn_glu, model.c:14-25;
  * with LLAMINI_ACT_NONE and no up, the rounding of plain rows to int8), q and
- * scale of y. gate and up are of `type` and may lie side by side in one buffer,
+ * scale of y. act(x) is x / (1 + exp(-z)) in f32 (z = x for SiLU, 2 u for GELU's
+ * 1 + tanh u), zero where 1 + exp(-z) passes f32's range (z below -88.7). gate and up are of `type` and may lie side by side in one buffer,
  * as one product of both matrices leaves them. */
 int llamini_glu_i8_device(u32 type, const void* d_gate, u64 ld_gate, const void* d_up, u64 ld_up, u32 act,
                           u32 rows, u32 cols, i8* d_q, u64 ld_q, f32* d_scale, void* stream);

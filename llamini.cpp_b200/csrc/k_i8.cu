@@ -153,27 +153,30 @@ struct GluArgs {
     uint32_t rows, cols, act;
 };
 
-// The activations of model.c:14-25 (and gpt2.c's gelu), in f32, as x / (1 +
-// exp(-z)): SiLU's z is x; GELU's (1 + tanh u) / 2 is 1 / (1 + exp(-2 u)), which
-// does not cancel for negative u. exp(-z) is 2^(-z log2 e) with the factor folded
-// into z's constants: its argument's rounding leaves a relative error of up to
-// |z| 2^-24, next to the 2^-22 of the two approximate instructions, where the
-// result is rounded to 8 bits. 26 instructions an element became 14 (4096 x 11008
-// bf16: 58 us with expf and an exact division).
-__device__ __forceinline__ float sigmoid_of(float minus_z_log2e) {
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(e) : "f"(minus_z_log2e));
-    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(1.0f + e));
-    return r;
+// The activations of model.c:14-25 (and gpt2.c's gelu) times up, in f32, as
+// x up / (1 + exp(-z)): SiLU's z is x; GELU's (1 + tanh u) / 2 is 1 / (1 + exp(-2 u)),
+// which does not cancel for negative u. With h = exp(-z / 2) = 2^(-z log2 e / 2), the
+// factor folded into z's constants, 1 / (1 + h h) is the square of a reciprocal root s,
+// and x and up take one s each: where h h nears f32's limit (z = -88.7, beyond which
+// 1 + exp(-z) is infinite and the result 0, as in model.c) the reciprocal itself would
+// already be below f32's normal numbers, its root is far from there. Two approximate
+// instructions, each of relative error 2^-22 that the squares double, and where h h
+// counts (z < 0) |z| 2^-23 for SiLU from the argument's rounding (the product and the
+// constant) and |z| 2^-22 for GELU (x x, the fused sum, the product and two constants), next
+// to a result that is rounded to 8 bits. 26 instructions an element became 15 (4096 x
+// 11008 bf16: 58 us with expf and an exact division).
+__device__ __forceinline__ float root_sigmoid(float minus_half_z_log2e) {
+    float h, s;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(h) : "f"(minus_half_z_log2e));
+    asm("rsqrt.approx.ftz.f32 %0, %1;\n" : "=f"(s) : "f"(fmaf(h, h, 1.0f)));
+    return s;
 }
-__device__ __forceinline__ float activate(float x, uint32_t act) {
+__device__ __forceinline__ float activate(float x, float up, uint32_t act) {
     constexpr float log2e = 1.4426950408889634f;
-    if (act == ACT_SILU) return x * sigmoid_of(x * -log2e);
-    if (act == ACT_GELU) {
-        constexpr float k = -2.0f * 0.79788456080286535587989211986876f * log2e;
-        return x * sigmoid_of(x * fmaf(0.044715f * k, x * x, k));
-    }
-    return x;
+    if (act == LLAMINI_ACT_NONE) return x * up;
+    constexpr float k = -0.79788456080286535587989211986876f * log2e;
+    const float s = root_sigmoid(act == ACT_SILU ? x * (-0.5f * log2e) : x * fmaf(0.044715f * k, x * x, k));
+    return (x * s) * (up * s);
 }
 
 template <typename T>
@@ -185,20 +188,21 @@ __global__ void __launch_bounds__(512) glu_i8_kernel(const GluArgs a) {
     uint32_t m = 0;
     float unused = 0.f;
     for (uint32_t i = threadIdx.x; i < a.cols; i += blockDim.x)
-        m = max(m, abs_bits(activate(to_f32(g[i]), a.act) * (u ? to_f32(u[i]) : 1.f)));
+        m = max(m, abs_bits(activate(to_f32(g[i]), u ? to_f32(u[i]) : 1.f, a.act)));
     block_max_sum(m, unused, red);
     const RowScale s = row_scale(__uint_as_float(m));
     for (uint32_t i = threadIdx.x; i < a.cols; i += blockDim.x)
-        a.q[row * a.ld_q + i] = (int8_t)quant1(activate(to_f32(g[i]), a.act) * (u ? to_f32(u[i]) : 1.f), s);
+        a.q[row * a.ld_q + i] = (int8_t)quant1(activate(to_f32(g[i]), u ? to_f32(u[i]) : 1.f, a.act), s);
     if (threadIdx.x == 0) a.scale[row] = s.scale();
 }
 
 // The same with a row's values in the registers of G threads, read and
 // activated once; the next row's loads are in flight meanwhile. Bound by memory and
-// instruction issue (60 % of slots at bf16 4096 x 11008 SiLU: 42.6 us, 5.29 TB/s; f32
-// 2048 x 11008 32.8 us, 6.18 TB/s).
+// instruction issue (bf16 4096 x 11008 SiLU: 41.8 us, 5.39 TB/s; f32 2048 x 11008 33.1 us,
+// 6.13 TB/s). Four CTAs an SM where a warp has a row of one piece a lane: 20000 x 256
+// bf16 6.5 us, 7.3 with the three that more registers leave.
 template <typename T, bool UP, bool WARP, uint32_t E, uint32_t V>
-__global__ void __launch_bounds__(rows_threads<WARP, E, V, 16>(), V * E == 24 && V == 3 ? 2 : 1) glu_i8_rows_kernel(const GluArgs a) {
+__global__ void __launch_bounds__(rows_threads<WARP, E, V, 16>(), V * E == 24 && V == 3 ? 2 : WARP && V == 1 ? 4 : 1) glu_i8_rows_kernel(const GluArgs a) {
     constexpr uint32_t R = WARP ? kWarpRows : 1;
     constexpr bool AHEAD = rows_ahead<E, V>();
     __shared__ uint32_t red[WARP ? 1 : 128];
@@ -225,20 +229,20 @@ __global__ void __launch_bounds__(rows_threads<WARP, E, V, 16>(), V * E == 24 &&
 #pragma unroll
         for (uint32_t j = 0; j < V; j++) {
             piece_to_f32<T, E>(g[j], y[j]);
-            if (a.act == ACT_SILU) {                 // (one branch a piece, the same for all)
-#pragma unroll
-                for (uint32_t i = 0; i < E; i++) y[j][i] = activate(y[j][i], ACT_SILU);
-            } else if (a.act == ACT_GELU) {
-#pragma unroll
-                for (uint32_t i = 0; i < E; i++) y[j][i] = activate(y[j][i], ACT_GELU);
-            }
             float f[E];
             if (UP) piece_to_f32<T, E>(u[j], f);
+            if (a.act == ACT_SILU) {                 // (one branch a piece, the same for all)
 #pragma unroll
-            for (uint32_t i = 0; i < E; i++) {
-                if (UP) y[j][i] *= f[i];
-                top = max_abs(top, y[j][i]);
+                for (uint32_t i = 0; i < E; i++) y[j][i] = activate(y[j][i], UP ? f[i] : 1.f, ACT_SILU);
+            } else if (a.act == ACT_GELU) {
+#pragma unroll
+                for (uint32_t i = 0; i < E; i++) y[j][i] = activate(y[j][i], UP ? f[i] : 1.f, ACT_GELU);
+            } else if (UP) {
+#pragma unroll
+                for (uint32_t i = 0; i < E; i++) y[j][i] *= f[i];
             }
+#pragma unroll
+            for (uint32_t i = 0; i < E; i++) top = max_abs(top, y[j][i]);
         }
         if (AHEAD && row + step < a.rows) load(row + step);
         uint32_t m = abs_bits(top);

@@ -247,3 +247,63 @@ def test_weights_at_the_edge_of_shared_memory(gpu, orc):
 @pytest.mark.parametrize("cols,pad,shift", [(98304, 0, 0), (130816, 3, 2), (106752, 16, 14)])
 def test_weights_in_several_segments(gpu, orc, synth, t, cols, pad, shift):
     _check_weights(gpu, orc, synth, t, 3, cols, pad, shift)
+
+
+# ---------------------------------------------------------------- gated activation
+
+# gates in [low, high) times an `up` of this size: products of f32's range from gates far
+# below zero, down to where 1 + exp(-gate) leaves that range
+FAR = [(0, -12.0, -9.0, 1.0), (0, -88.5, -80.0, 1.0), (0, -88.5, -87.0, 1e30), (0, -88.5, -87.5, 1e37), (0, -70.0, -60.0, 1e-3),
+       (1, -8.0, -7.0, 1.0), (1, -10.2, -9.9, 1e36), (1, -9.5, -6.0, 1e3)]
+
+
+def _far_call(gpu, type, act, gate, up, rows, cols, pad):
+    gr, ur = Rows(rows, cols, DT[type], pad, fill=gate), Rows(rows, cols, DT[type], pad, fill=up)
+    q, scale = Rows(rows, cols, torch.int8, pad if pad else (-cols) % 16), torch.empty(rows, device="cuda")
+    base._ok(gpu, base._glu(gpu, type, gr, ur, act, rows, cols, q, scale))
+    torch.cuda.synchronize()
+    return gr.t, ur.t, q, scale
+
+
+@pytest.mark.parametrize("type", [0, 30])
+@pytest.mark.parametrize("act,low,high,size", FAR)
+@pytest.mark.parametrize("rows,cols,pad", [(4, 64, 0), (1100, 64, 0), (1100, 100, 1), (3, 4864, 0), (3, 777, 1), (2, 40000, 1)])
+def test_glu_of_gates_far_below_zero(gpu, type, act, low, high, size, rows, cols, pad):
+    g = base._gen(cols + rows)
+    gate = torch.rand(rows, cols, generator=g, device="cuda") * (high - low) + low
+    up = base._rand(g, rows, cols).sign() * (0.5 + torch.rand(rows, cols, generator=g, device="cuda")) * size
+    x, u, q, scale = _far_call(gpu, type, act, gate, up, rows, cols, pad)
+    x = x.double()
+    z = x if act == 0 else 2 * np.sqrt(2 / np.pi) * (x + 0.044715 * x ** 3)
+    y = x * torch.sigmoid(z) * u.double()
+    # zero where 1 + exp(-z) is past f32's largest number, z = -88.72; within z's own error
+    # of that (six roundings of 89: 3.2e-5) either
+    limit = -float(np.log(np.finfo(np.float32).max))
+    y = torch.where((z < limit) & ((z - limit).abs() > 1e-4) | ((z - limit).abs() <= 1e-4) & (q.t == 0), 0.0, y)
+    # the argument: |z| 2^-23 (SiLU), |z| 2^-22 (GELU); the squares of two approximations
+    # of 2^-22; eight roundings of products and sums
+    r = ((2 if act == 0 else 4) * float(z.abs().max()) + 4 * 4 + 8) * F24
+    base._check_int8(q.t, scale, y, r)
+    assert q.untouched_around()
+
+
+@pytest.mark.parametrize("type", [0, 30])
+@pytest.mark.parametrize("cols,pad", [(64, 0), (777, 1), (4864, 0), (40000, 1)])
+def test_glu_of_gates_whose_sigmoid_is_zero(gpu, type, cols, pad):
+    """Below -89 SiLU is zero in f32, as in ffn_glu: such gates count for nothing
+    beside others, and a row of them is a row of zeros."""
+    g = base._gen(cols)
+    gate = torch.rand(4, cols, generator=g, device="cuda") * -100 - 90
+    gate[2, cols // 2], gate[3, 0] = -20.0, 1.0
+    up = base._rand(g, 4, cols) * 1e6
+    x, u, q, scale = _far_call(gpu, type, 0, gate, up, 4, cols, pad)
+    host = [t.float().contiguous().cpu().numpy() for t in (x, u)]
+    for i in range(4):
+        out = np.empty(cols, np.float32)
+        gpu.lib().ffn_glu(gpu.ptr(out), gpu.ptr(host[0][i]), gpu.ptr(host[1][i]), cols, 0)
+        assert np.count_nonzero(out) == (0 if i < 2 else 1)
+    assert torch.all(scale[:2] == 0) and torch.all(q.t[:2] == 0)
+    for i, at in ((2, cols // 2), (3, 0)):
+        assert q.t[i].count_nonzero() == 1 and abs(int(q.t[i, at])) == 127
+        want = x[i, at].double() * torch.sigmoid(x[i, at].double()) * u[i, at].double()
+        assert abs(float(scale[i].double() * 127 / want.abs()) - 1) < 80 * F24      # |z| of 20
