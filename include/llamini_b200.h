@@ -135,7 +135,8 @@ int llamini_weights_i8_device(u32 type, const void* d_blocks, u32 rows, u32 cols
  * eps) * w (rms_norm, model.c:4-10), q and scale of y. x, resid and sum are of
  * `type`. d_sum (NULL: not stored) receives h rounded to `type`; it may be d_x or
  * d_resid, with that input's pitch, to update a residual stream in place. d_w
- * holds `cols` floats. */
+ * holds `cols` floats. A row whose sum of squares passes f32's range (finite values past
+ * 1e19, say), or whose mean(h^2) + eps is below 2^-120, has scale NaN and q = 0. */
 int llamini_rms_norm_i8_device(u32 type, const void* d_x, u64 ld_x, const void* d_resid, u64 ld_resid,
                                void* d_sum, u64 ld_sum, const f32* d_w, f32 eps, u32 rows, u32 cols,
                                i8* d_q, u64 ld_q, f32* d_scale, void* stream);

@@ -37,6 +37,18 @@ struct NormArgs {
     float eps;
 };
 
+// 1 / sqrt(mean + eps) of a row's sum of squares. Squares leave f32's range long before
+// the values do (|h| of 1.8e19; with an eps of next to nothing 1e-18 below): a sum that
+// is infinite, or so small that its squares were rounded to multiples of 2^-149 that
+// count, gives NaN, and the row's scale with it, instead of zeros or a wrong size. (Such
+// rows summed again with scaled values cost the others 5 to 30 %: 1 x 2048 f32 1.7 -> 2.3
+// us, 4096 x 4096 bf16 20.8 -> 22.1.)
+constexpr float kLeastMean = 0x1p-120f;
+__device__ __forceinline__ float rms_recip(float ss, uint32_t cols, float eps) {
+    const float v = ss / (float)cols + eps;
+    return v >= kLeastMean && v < INFINITY ? 1.0f / sqrtf(v) : NAN;
+}
+
 // h = x + resid in f32 (its rounding to the type is only for the stored sum),
 // y = h / sqrt(mean(h^2) + eps) * w. One CTA a row. Each thread reads an
 // element before the same thread overwrites it, in the second pass, so the sum
@@ -56,7 +68,7 @@ __global__ void __launch_bounds__(512) norm_i8_kernel(const NormArgs a) {
         m = max(m, abs_bits(h * a.w[i]));
     }
     block_max_sum(m, ss, red);
-    const float rstd = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
+    const float rstd = rms_recip(ss, a.cols, a.eps);
     const RowScale s = row_scale(__uint_as_float(m) * rstd);
     for (uint32_t i = threadIdx.x; i < a.cols; i += blockDim.x) {
         const float h = to_f32(x[i]) + (r ? to_f32(r[i]) : 0.f);
@@ -126,7 +138,7 @@ __global__ void __launch_bounds__(rows_threads<WARP, E, V, 8>()) norm_i8_rows_ke
         if (AHEAD && row + step < a.rows) load(row + step);
         uint32_t m = abs_bits(top);
         row_max_sum<WARP>(m, ss, red, turn);
-        const float rstd = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
+        const float rstd = rms_recip(ss, a.cols, a.eps);
         const RowScale s = row_scale(__uint_as_float(m) * rstd);
         float f = rstd * s.inv;
         if (!(s.plain && f < INFINITY)) {            // in two steps

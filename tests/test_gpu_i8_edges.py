@@ -307,3 +307,79 @@ def test_glu_of_gates_whose_sigmoid_is_zero(gpu, type, cols, pad):
         assert q.t[i].count_nonzero() == 1 and abs(int(q.t[i, at])) == 127
         want = x[i, at].double() * torch.sigmoid(x[i, at].double()) * u[i, at].double()
         assert abs(float(scale[i].double() * 127 / want.abs()) - 1) < 80 * F24      # |z| of 20
+
+
+# ---------------------------------------------------------------- norm
+
+# sizes of a row's values and eps: sums of squares below, at and past f32's largest number,
+# and means past the least that the norm takes
+SIZES = [(1e20, 1e-5), (3e37, 1e-5), (1e18, 1e-5), (1e15, 1e-6), (1e-16, 0.0), (1e-21, 0.0), (1e-37, 0.0), (1e-18, 1e-35), (1e-30, 1e-30),
+         (1.0, 0.0)]
+
+
+def _range_of(h, eps):
+    """Rows whose mean of squares f32 holds, and those that it does not (the sums of
+    no row here lie so close to a limit that the order of its additions decides)."""
+    ss = h.square().sum(dim=1)
+    mean = ss / h.shape[1] + eps
+    top, least = float(np.finfo(np.float32).max), 2.0 ** -120
+    assert torch.all((ss / top - 1).abs() > 1e-3) and torch.all((mean / least - 1).abs() > 1e-3)
+    fine = (ss < top) & (mean > least)
+    return fine, ~fine
+
+
+@pytest.mark.parametrize("type", [0, 30])
+@pytest.mark.parametrize("size,eps", SIZES)
+@pytest.mark.parametrize("rows,cols,pad,resid", [(3, 64, 0, False), (1100, 64, 0, True), (1100, 100, 1, True), (3, 4096, 0, True), (5, 777, 1, False),
+                                                 (2, 11008, 0, True), (3, 12000, 1, True), (1100, 8192, 0, True), (2, 40000, 0, False)])
+def test_norm_of_rows_of_any_size(gpu, type, size, eps, rows, cols, pad, resid):
+    """Large and tiny rows, some with a part of ordinary size, beside an ordinary
+    one: right, or where a mean leaves f32's range a scale of NaN."""
+    g = base._gen(cols + rows)
+    x0 = base._rand(g, rows, cols).clamp_(-5, 5) * size
+    x0[0] = base._rand(g, cols)                    # an ordinary row
+    x0[1, 1:cols // 2] = 0.0
+    if size > 1:
+        x0[-1, cols // 2:] = 1.0
+    x = Rows(rows, cols, DT[type], pad, fill=x0)
+    r = Rows(rows, cols, DT[type], pad, fill=base._rand(g, rows, cols) * size / 4) if resid else None
+    out = Rows(rows, cols, DT[type], pad) if resid else None
+    w = 1 + base._rand(g, cols, scale=0.05)
+    q, scale = Rows(rows, cols, torch.int8, pad if pad else (-cols) % 16), torch.empty(rows, device="cuda")
+    base._ok(gpu, base._norm(gpu, type, x, r, out, w, eps, rows, cols, q, scale))
+    torch.cuda.synchronize()
+    h = x.t.double() + (r.t.double() if resid else 0)
+    eps = float(np.float32(eps))
+    fine, lost = _range_of(h, eps)
+    assert torch.isnan(scale[lost]).all() and torch.all(q.t[lost] == 0)
+    y = h / (h.square().mean(dim=1, keepdim=True) + eps).sqrt() * w.double()
+    # a square is off by up to 2^-150 beside means of 2^-120 and more
+    base._check_int8(q.t[fine], scale[fine], y[fine], base._norm_r(cols) + 2.0 ** -30)
+    assert q.untouched_around()
+    if resid:
+        half = torch.finfo(DT[type]).eps / 2 + F24
+        assert torch.all((out.t.double() - h).abs() <= h.abs() * half + 2.0 ** -149)
+
+
+@pytest.mark.parametrize("type", [0, 30])
+@pytest.mark.parametrize("rows,cols", [(40, 64), (2000, 100), (300, 2048), (1100, 4096), (700, 20000)])
+def test_norm_of_large_rows_among_others(gpu, type, rows, cols):
+    """Every third row is too large: CTAs and warps that walk over rows go from one
+    kind to the other, and the ordinary rows keep the bits that they have alone."""
+    g = base._gen(rows)
+    x0 = base._rand(g, rows, cols)
+    plain = Rows(rows, cols, DT[type], fill=x0)
+    x0[::3] *= 1e25
+    x0[::6, : cols // 3] = 2.0
+    mixed = Rows(rows, cols, DT[type], fill=x0)
+    w = 1 + base._rand(g, cols, scale=0.05)
+    got = []
+    for x in (plain, mixed):
+        q, scale = Rows(rows, cols, torch.int8, (-cols) % 16), torch.empty(rows, device="cuda")
+        base._ok(gpu, base._norm(gpu, type, x, None, None, w, 1e-5, rows, cols, q, scale))
+        got.append((q.t, scale))
+    others = torch.arange(rows, device="cuda") % 3 != 0
+    assert torch.equal(got[0][0][others], got[1][0][others]) and torch.equal(got[0][1][others], got[1][1][others])
+    assert torch.isnan(got[1][1][~others]).all() and torch.all(got[1][0][~others] == 0)
+    h = plain.t.double()
+    base._check_int8(*got[0], h / (h.square().mean(1, True) + float(np.float32(1e-5))).sqrt() * w.double(), base._norm_r(cols))
