@@ -50,7 +50,7 @@ constexpr uint32_t kST = 64, kSK = 64, kSW = kSK / 4, kSPad = kSW + 4, kSN = kST
 
 // The words of this thread of 64 rows x kSK columns from row r0, column k0 on;
 // zeros past the matrix. A word at any address comes from the two aligned words
-// around it, each of which holds a byte of the row.
+// around it, which begin up to 3 bytes before it and end at most 8 behind its start.
 __device__ __forceinline__ void fetch_words(uint32_t* v, const int8_t* src, uint64_t ld, uint32_t r0, uint32_t rows, uint32_t k0,
                                             uint32_t k) {
 #pragma unroll
@@ -59,7 +59,7 @@ __device__ __forceinline__ void fetch_words(uint32_t* v, const int8_t* src, uint
         v[j] = 0;
         if (r0 + r >= rows) continue;
         const uint8_t* p = reinterpret_cast<const uint8_t*>(src) + (uint64_t)(r0 + r) * ld + c;
-        if (c + 7 <= k) {
+        if (c + 8 <= k) {
             const uintptr_t a = reinterpret_cast<uintptr_t>(p);
             const uint32_t* w = reinterpret_cast<const uint32_t*>(a & ~uintptr_t(3));
             v[j] = __funnelshift_r(w[0], w[1], (uint32_t)(a & 3u) * 8u);
@@ -164,13 +164,14 @@ enum RowsAt : uint32_t { ROWS_WHOLE, ROWS_TAIL, ROWS_ANY };
 // Vector v (16 bytes) of a row of k bytes, read once by the device (STREAM: the
 // weights) or by every CTA: zeros past its end. Nothing behind the
 // row is read; a row at any address is read in the aligned words around the
-// vector, up to 3 bytes before the row's own first.
+// vector (up to 3 bytes before the row's own first), which end at most 20 bytes behind
+// the vector's start.
 template <uint32_t AT, bool STREAM>
 __device__ __forceinline__ uint4 row_vec(const uint8_t* row, uint32_t v, uint32_t k) {
     const uint32_t at = 16 * v;
     const uint8_t* p = row + at;
     if (AT == ROWS_ANY) {
-        if (at + 19 <= k) {
+        if (at + 20 <= k) {
             const uintptr_t a = reinterpret_cast<uintptr_t>(p);
             const uint32_t* b = reinterpret_cast<const uint32_t*>(a & ~uintptr_t(3));
             const uint32_t s = (uint32_t)(a & 3u) * 8u;

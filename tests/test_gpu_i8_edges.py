@@ -197,6 +197,24 @@ def test_status_of_a_stream_in_capture_is_refused(gpu):
     base._ok(gpu, L.llamini_i8_status(base._stream()))
 
 
+@pytest.mark.parametrize("m", [1, 5, 20, 600])
+@pytest.mark.parametrize("k", [3, 7, 8, 19, 20, 35, 67, 71, 72, 131])
+@pytest.mark.parametrize("shift", range(4))
+def test_rows_that_end_with_the_last_word(gpu, m, k, shift):
+    """Rows at every alignment whose last whole vector or word ends where the row does,
+    or a byte or two before: the last row is the last of its buffer."""
+    n = 650
+    a, w, sa, sw, b, call = _product(gpu, m, n, k, 0, k)
+    out = Rows(m, n, torch.float32)
+    tight = [torch.empty(shift + x.rows * k, dtype=torch.int8, device="cuda") for x in (a, w)]
+    for t, x in zip(tight, (a, w)):
+        t[shift:].view(x.rows, k).copy_(x.t)
+    base._ok(gpu, gpu.lib().llamini_gemm_i8_device(tight[0].data_ptr() + shift, k, sa.data_ptr(), m, tight[1].data_ptr() + shift, k,
+                                                   sw.data_ptr(), n, k, b.data_ptr(), 0, out.ptr, out.ld, base._stream()))
+    torch.cuda.synchronize()
+    base._check_gemm(out.t, 0, a.t, sa, w.t, sw, b)
+
+
 # ---------------------------------------------------------------- weights
 
 BLOCK = {2: (32, 18), 3: (32, 20), 6: (32, 22), 8: (32, 34), 12: (256, 144), 13: (256, 176), 14: (256, 210)}
