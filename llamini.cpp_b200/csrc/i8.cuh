@@ -32,10 +32,10 @@ inline size_t act_bytes(uint32_t type) {
     return type == GGML_TYPE_F32 ? 4 : type == GGML_TYPE_F16 || type == LLAMINI_TYPE_BF16 ? 2 : 0;
 }
 
-// Whether every pointer of ptrs[0..n) (null ones are skipped) is memory that a
+// Whether every pointer of ptrs[0..n), called names[0..n) (null ones are skipped), is memory that a
 // kernel on the calling thread's current device may use: that device's own, or
 // managed. A host pointer, or another device's, would fault in the kernel.
-inline bool i8_device_ptrs(const char* who, const void* const* ptrs, int n) {
+inline bool i8_device_ptrs(const char* who, const void* const* ptrs, const char* const* names, int n) {
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess) {
         cudaGetLastError();
@@ -48,7 +48,7 @@ inline bool i8_device_ptrs(const char* who, const void* const* ptrs, int n) {
         if (!LM_CUDA(cudaPointerGetAttributes(&a, ptrs[i]))) return false;
         if (a.type == cudaMemoryTypeManaged) continue;
         if (a.type != cudaMemoryTypeDevice || a.device != dev) {
-            set_error("%s: pointer argument %d is not memory of the current device (%d)", who, i + 1, dev);
+            set_error("%s: %s is not memory of the current device (%d)", who, names[i], dev);
             return false;
         }
     }

@@ -1208,7 +1208,8 @@ extern "C" int llamini_gemm_i8_device(const i8* d_a, u64 ld_a, const f32* d_a_sc
         return -1;
     }
     const void* ptrs[] = {d_a, d_a_scale, d_w, d_w_scale, d_bias, d_out};
-    if (!i8_device_ptrs(who, ptrs, 6)) return -1;
+    const char* const names[] = {"a", "a_scale", "w", "w_scale", "bias", "out"};
+    if (!i8_device_ptrs(who, ptrs, names, 6)) return -1;
     GemmI8Args g;
     g.a = reinterpret_cast<const int8_t*>(d_a); g.as = d_a_scale;
     g.w = reinterpret_cast<const int8_t*>(d_w); g.ws = d_w_scale;
@@ -1225,8 +1226,7 @@ extern "C" int llamini_gemm_i8_device(const i8* d_a, u64 ld_a, const f32* d_a_sc
 extern "C" int llamini_i8_status(void* stream) {
     using namespace lm;
     const char* who = "i8_status";
-    const void* none[1] = {nullptr};
-    if (!i8_device_ptrs(who, none, 1)) return -1;
+    if (!i8_device_ptrs(who, nullptr, nullptr, 0)) return -1;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     if (!LM_CUDA(cudaStreamIsCapturing(st, &capture))) return -1;

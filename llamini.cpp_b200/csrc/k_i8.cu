@@ -753,9 +753,10 @@ extern "C" int llamini_weights_i8_device(u32 type, const void* d_blocks, u32 row
     }
     if (rows == 0) return 0;
     const void* ptrs[] = {d_blocks, d_q, d_scale};
+    const char* const names[] = {"blocks", "q", "scale"};
     if (!d_blocks || !d_q || !d_scale) { set_error("%s: null pointer", who); return -1; }
     const size_t align = type == GGML_TYPE_F32 ? 4 : 2;      // blocks start with, and are read in, 16-bit fields
-    if (!align_ok(who, ptrs, 1, align) || !align_ok(who, ptrs + 2, 1, 4) || !i8_device_ptrs(who, ptrs, 3)) return -1;
+    if (!align_ok(who, ptrs, 1, align) || !align_ok(who, ptrs + 2, 1, 4) || !i8_device_ptrs(who, ptrs, names, 3)) return -1;
     WeightArgs a;
     a.raw = static_cast<const uint8_t*>(d_blocks);
     a.q = reinterpret_cast<int8_t*>(d_q);
@@ -801,9 +802,10 @@ extern "C" int llamini_rms_norm_i8_device(u32 type, const void* d_x, u64 ld_x, c
     }
     if (rows == 0) return 0;
     const void* ptrs[] = {d_x, d_resid, d_sum, d_w, d_q, d_scale};
+    const char* const names[] = {"x", "resid", "sum", "w", "q", "scale"};
     if (!d_x || !d_w || !d_q || !d_scale) { set_error("%s: null pointer", who); return -1; }
     const void* f32s[] = {d_w, d_scale};
-    if (!align_ok(who, ptrs, 3, act_bytes(type)) || !align_ok(who, f32s, 2, 4) || !i8_device_ptrs(who, ptrs, 6)) return -1;
+    if (!align_ok(who, ptrs, 3, act_bytes(type)) || !align_ok(who, f32s, 2, 4) || !i8_device_ptrs(who, ptrs, names, 6)) return -1;
     NormArgs a;
     a.x = d_x; a.resid = d_resid; a.sum = d_sum; a.w = d_w;
     a.q = reinterpret_cast<int8_t*>(d_q); a.scale = d_scale;
@@ -826,8 +828,9 @@ extern "C" int llamini_glu_i8_device(u32 type, const void* d_gate, u64 ld_gate, 
     if (act > LLAMINI_ACT_NONE) { set_error("%s: unknown activation %u", who, act); return -1; }
     if (rows == 0) return 0;
     const void* ptrs[] = {d_gate, d_up, d_q, d_scale};
+    const char* const names[] = {"gate", "up", "q", "scale"};
     if (!d_gate || !d_q || !d_scale) { set_error("%s: null pointer", who); return -1; }
-    if (!align_ok(who, ptrs, 2, act_bytes(type)) || !align_ok(who, ptrs + 3, 1, 4) || !i8_device_ptrs(who, ptrs, 4)) return -1;
+    if (!align_ok(who, ptrs, 2, act_bytes(type)) || !align_ok(who, ptrs + 3, 1, 4) || !i8_device_ptrs(who, ptrs, names, 4)) return -1;
     GluArgs a;
     a.gate = d_gate; a.up = d_up;
     a.q = reinterpret_cast<int8_t*>(d_q); a.scale = d_scale;

@@ -401,3 +401,26 @@ def test_norm_of_large_rows_among_others(gpu, type, rows, cols):
     assert torch.isnan(got[1][1][~others]).all() and torch.all(got[1][0][~others] == 0)
     h = plain.t.double()
     base._check_int8(*got[0], h / (h.square().mean(1, True) + float(np.float32(1e-5))).sqrt() * w.double(), base._norm_r(cols))
+
+
+# ---------------------------------------------------------------- refusals
+
+def test_refusals_name_the_array(gpu):
+    """One host array among device arrays: the message says which."""
+    L, d = gpu.lib(), torch.zeros(8192, device="cuda").data_ptr()
+    h = np.zeros(8192, np.float32)
+
+    def each(call, names):
+        for at, name in enumerate(names):
+            args = [d] * len(names)
+            args[at] = h.ctypes.data
+            L.llamini_clear_error()
+            assert call(*args) == -1
+            assert ": %s is not memory of the current device" % name in gpu.last_error()
+        L.llamini_clear_error()
+    each(lambda b, q, s: L.llamini_weights_i8_device(8, b, 4, 64, q, 64, s, None), ["blocks", "q", "scale"])
+    each(lambda x, r, o, w, q, s: L.llamini_rms_norm_i8_device(0, x, 64, r, 64, o, 64, w, 1e-5, 4, 64, q, 64, s, None),
+         ["x", "resid", "sum", "w", "q", "scale"])
+    each(lambda g, u, q, s: L.llamini_glu_i8_device(0, g, 64, u, 64, 0, 4, 64, q, 64, s, None), ["gate", "up", "q", "scale"])
+    each(lambda a, sa, w, sw, b, o: L.llamini_gemm_i8_device(a, 64, sa, 4, w, 64, sw, 8, 64, b, 0, o, 8, None),
+         ["a", "a_scale", "w", "w_scale", "bias", "out"])
