@@ -403,6 +403,61 @@ def test_norm_of_large_rows_among_others(gpu, type, rows, cols):
     base._check_int8(*got[0], h / (h.square().mean(1, True) + float(np.float32(1e-5))).sqrt() * w.double(), base._norm_r(cols))
 
 
+# ---------------------------------------------------------------- long walks
+#
+# More rows than CTAs run at once, so that each CTA goes through several: buffers and
+# halves of shared memory that alternate, the next row's loads under way.
+
+@pytest.mark.parametrize("t,rows,cols", [(2, 4096, 2048), (3, 9000, 256), (6, 4096, 2048), (8, 4096, 2048), (8, 20000, 96), (8, 700, 20480),
+                                         (12, 9000, 768), (12, 700, 20480), (13, 4096, 2048), (14, 4096, 2048), (14, 2000, 5632)])
+def test_weights_of_many_rows(gpu, orc, synth, t, rows, cols):
+    _check_weights(gpu, orc, synth, t, rows, cols)
+
+
+# vectors a thread: 1, 2, 3, 4, 6, 8 of eight elements and of four; then one element at a time
+WALKS = [(1200, 2048), (1000, 4096), (1100, 4096), (700, 11008), (700, 14336), (500, 20480), (400, 30000), (1200, 5632), (1200, 7168),
+         (3000, 500), (700, 3001), (500, 12001)]
+
+
+@pytest.mark.parametrize("type", [0, 1, 30])
+@pytest.mark.parametrize("rows,cols", WALKS)
+@pytest.mark.parametrize("resid", [False, True])
+def test_norm_of_many_rows(gpu, type, rows, cols, resid):
+    g = base._gen(rows + cols)
+    pad = (-cols) % 8 if cols % 8 == 4 else 0
+    x = Rows(rows, cols, DT[type], pad, fill=base._rand(g, rows, cols))
+    r0 = base._rand(g, rows, cols, scale=3)
+    r = Rows(rows, cols, DT[type], pad, fill=r0) if resid else None
+    w = 1 + base._rand(g, cols, scale=0.05)
+    q, scale = Rows(rows, cols, torch.int8, pad), torch.empty(rows, device="cuda")
+    h = x.t.double() + (r.t.double() if resid else 0)
+    base._ok(gpu, base._norm(gpu, type, x, r, r, w, 1e-5, rows, cols, q, scale))      # the sum over the residual
+    torch.cuda.synchronize()
+    y = h / (h.square().mean(dim=1, keepdim=True) + float(np.float32(1e-5))).sqrt() * w.double()
+    base._check_int8(q.t, scale, y, base._norm_r(cols))
+    assert q.untouched_around()
+    if resid:
+        half = torch.finfo(DT[type]).eps / 2 + F24
+        assert torch.all((r.t.double() - h).abs() <= h.abs() * half + 2.0 ** -25) and r.untouched_around()
+
+
+@pytest.mark.parametrize("type", [0, 1, 30])
+@pytest.mark.parametrize("rows,cols", WALKS + [(1500, 9000), (2000, 11008)])
+@pytest.mark.parametrize("act,with_up", [(0, True), (2, False)])
+def test_glu_of_many_rows(gpu, type, rows, cols, act, with_up):
+    g = base._gen(rows + cols)
+    pad = (-cols) % 8 if cols % 8 == 4 else 0
+    gate = Rows(rows, cols, DT[type], pad, fill=base._rand(g, rows, cols, scale=3))
+    up = Rows(rows, cols, DT[type], pad, fill=base._rand(g, rows, cols)) if with_up else None
+    q, scale = Rows(rows, cols, torch.int8, pad), torch.empty(rows, device="cuda")
+    base._ok(gpu, base._glu(gpu, type, gate, up, act, rows, cols, q, scale))
+    torch.cuda.synchronize()
+    y = base._act64(gate.t.double(), act) * (up.t.double() if with_up else 1.0)
+    # SiLU of gates down to 3 x 6: argument 18 x 2^-23, approximations 2 x 2 x 2^-22, roundings
+    base._check_int8(q.t, scale, y, (36 + 16 + 8) * F24 if act == 0 else 4 * F24)
+    assert q.untouched_around()
+
+
 # ---------------------------------------------------------------- refusals
 
 def test_refusals_name_the_array(gpu):
