@@ -168,7 +168,8 @@ int llamini_set_i8_wait_ns(u64 ns);
  * run out on the current device, on this stream or another, since the last call for
  * this stream (for its first: since the library was loaded). The outputs of such a
  * product are NaN; a call for one stream takes nothing away from another's. A
- * stream that is being captured is refused, and its capture goes on. */
+ * stream that is being captured is refused, and its capture goes on; so do the captures
+ * of other streams. */
 int llamini_i8_status(void* stream);
 
 /* ---- device-resident decoding sessions (generate.c:122-167 without host

@@ -1234,10 +1234,14 @@ extern "C" int llamini_i8_status(void* stream) {
     int dev = 0;
     unsigned long long id = 0;                       // of the stream; no later one has it again
     uint32_t count = 0;
-    if (!LM_CUDA(cudaGetDevice(&dev)) || !LM_CUDA(cudaStreamGetId(st, &id)) || !LM_CUDA(cudaStreamSynchronize(st)) ||
-        !LM_CUDA(cudaMemcpyFromSymbolAsync(&count, g_i8_err, sizeof(count), 0, cudaMemcpyDeviceToHost, st)) ||
-        !LM_CUDA(cudaStreamSynchronize(st)))
-        return -1;
+    // Another stream may be in a capture that forbids a wait to every stream and thread,
+    // and would end with it: this thread says that its calls have nothing to do with it.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if (!LM_CUDA(cudaThreadExchangeStreamCaptureMode(&mode))) return -1;
+    const bool ok = LM_CUDA(cudaGetDevice(&dev)) && LM_CUDA(cudaStreamGetId(st, &id)) && LM_CUDA(cudaStreamSynchronize(st)) &&
+                    LM_CUDA(cudaMemcpyFromSymbolAsync(&count, g_i8_err, sizeof(count), 0, cudaMemcpyDeviceToHost, st)) &&
+                    LM_CUDA(cudaStreamSynchronize(st));
+    if (!LM_CUDA(cudaThreadExchangeStreamCaptureMode(&mode)) || !ok) return -1;
     bool same = false;
     try {
         static std::mutex mu;

@@ -458,6 +458,63 @@ def test_glu_of_many_rows(gpu, type, rows, cols, act, with_up):
     assert q.untouched_around()
 
 
+# ---------------------------------------------------------------- first calls
+
+def first_calls_in_a_capture(gpu, synth):
+    """Each operator and product kernel for the first time in its process, inside a
+    capture; the replay, and the same calls made directly."""
+    L = gpu.lib()
+    e = dict(device="cuda")
+    n, k = 1024, 768
+    raws = [torch.from_numpy(synth.random_blocks(np.random.default_rng(t), t, n * k).copy()).cuda() for t in (8, 12)]
+    wide = torch.from_numpy(synth.random_blocks(np.random.default_rng(9), 8, 2 * 98304).copy()).cuda()
+    x = base._rand(base._gen(1), 900, k).bfloat16()
+    w = torch.ones(k, **e)
+    other = torch.cuda.Stream()
+
+    def run(st):
+        outs = []
+        for raw, t in zip(raws, (8, 12)):
+            q, s = torch.zeros(n, k, dtype=torch.int8, **e), torch.zeros(n, **e)
+            base._ok(gpu, L.llamini_weights_i8_device(t, raw.data_ptr(), n, k, q.data_ptr(), k, s.data_ptr(), st))
+            outs += [q, s]
+        q, s = torch.zeros(2, 98304, dtype=torch.int8, **e), torch.zeros(2, **e)
+        base._ok(gpu, L.llamini_weights_i8_device(8, wide.data_ptr(), 2, 98304, q.data_ptr(), 98304, s.data_ptr(), st))
+        outs += [q, s]
+        for m in (1, 40, 900):
+            a, sa = torch.zeros(m, k, dtype=torch.int8, **e), torch.zeros(m, **e)
+            h, sh = torch.zeros(m, n // 2, dtype=torch.int8, **e), torch.zeros(m, **e)
+            y = torch.zeros(m, n, dtype=torch.bfloat16, **e)
+            base._ok(gpu, L.llamini_rms_norm_i8_device(30, x.data_ptr(), k, None, 0, None, 0, w.data_ptr(), 1e-5, m, k, a.data_ptr(), k,
+                                                       sa.data_ptr(), st))
+            base._ok(gpu, L.llamini_gemm_i8_device(a.data_ptr(), k, sa.data_ptr(), m, outs[0].data_ptr(), k, outs[1].data_ptr(), n, k, None,
+                                                   30, y.data_ptr(), n, st))
+            base._ok(gpu, L.llamini_glu_i8_device(30, y.data_ptr(), n, y.data_ptr() + n, n, 0, m, n // 2, h.data_ptr(), n // 2,
+                                                  sh.data_ptr(), st))
+            outs += [a, sa, y, h, sh]
+        return outs
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run(base._stream())
+        base._ok(gpu, L.llamini_i8_status(other.cuda_stream))      # of a stream that is not captured
+    graph.replay()
+    torch.cuda.synchronize()
+    direct = run(base._stream())
+    torch.cuda.synchronize()
+    assert all(torch.equal(c, d) for c, d in zip(captured, direct))
+    assert all(c.float().abs().sum() > 0 for c in captured)
+
+
+def test_first_calls_in_a_capture(gpu):
+    code = ("import sys; sys.path[:0] = %r\n"
+            "import conftest, tiny, test_gpu_i8_edges as t\n"
+            "t.first_calls_in_a_capture(conftest._load_pkg(), tiny.synthetic())\n"
+            % [os.path.dirname(__file__), conftest.GOLDEN, os.path.join(conftest.ROOT, "oracle")])
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
 # ---------------------------------------------------------------- refusals
 
 def test_refusals_name_the_array(gpu):
