@@ -103,8 +103,11 @@ int llamini_causal_mha_noalloc(const f32* d_q, const f32* d_key, const f32* d_va
  * weights with one scale for each output channel, activations with one scale
  * for each token. A row q[0..cols) with its scale stands for the values
  * q[i] * scale, where scale = max|y| / 127 and q = y * (127 / max|y|) rounded to
- * the nearest integer, ties to even (both quotients rounded to f32). A row of
- * zeros has scale 0; a row that holds a NaN or an infinity has scale NaN and q = 0.
+ * the nearest integer, ties to even (both quotients rounded to f32; the norm rounds
+ * the factor once more, so that an element within 2^-16 of halfway may go the other
+ * way, and its sums' order, with it their last bits, goes by the rows' length, number
+ * and layout). A row of zeros has scale 0; a row that holds a NaN or an infinity has
+ * scale NaN and q = 0.
  *
  * Every call takes DEVICE buffers of the calling thread's current device (others
  * are refused) and enqueues its work on `stream` (a cudaStream_t; NULL = the

@@ -6,11 +6,15 @@
 // scale = max|y| / 127 and q = y * (127 / max|y|) rounded to the nearest integer,
 // ties to even, both quotients rounded to f32, so |q| <= 127 and -128 never
 // appears. (The reciprocal instead of y / scale moves only an element that lies
-// within 2^-16 of halfway between two integers, and makes the rounding of y one
-// fused multiply-add, exact and the same everywhere.) A row of zeros has scale 0.
+// within 2^-16 of halfway between two integers, among them exact ties, which it
+// takes either way -- a Q8_0 row whose largest code is -128 has them at its block's
+// +-64 -- and makes the rounding of y one fused multiply-add, the same everywhere. The
+// norm's row kernels fold 1 / rms into the factor, one rounding more.) A row of
+// zeros has scale 0.
 // A row that holds a NaN or an infinity has scale NaN and q = 0: every value it
-// stands for is NaN, so the fault stays visible. Where 127 / max|y| would
-// overflow (max|y| below 1.5e-36) y and max|y| are multiplied by 2^100 first.
+// stands for is NaN, so the fault stays visible. Where 127 / max|y| comes
+// near f32's limit (it passes it below a max|y| of 3.7e-37; the change is at 1.5e-36) y
+// and max|y| are multiplied by 2^100 first; where the scale rounds to 0 so does q.
 #pragma once
 
 #include "internal.h"

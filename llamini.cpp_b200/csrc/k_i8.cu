@@ -279,7 +279,7 @@ struct WeightArgs {
     int8_t* q;
     float* scale;
     uint64_t row_bytes, ld_q;
-    uint32_t rows, cols, type;
+    uint32_t rows, cols;
     uint32_t seg_units;        // units of a segment of a row that fits shared memory
 };
 
@@ -472,9 +472,10 @@ __global__ void __launch_bounds__(kWThreads) weights_i8_kernel(const WeightArgs 
 // The same for rows that fit: a CTA walks groups of rows (back to back in memory),
 // copies the next group's bytes while it works on this one's, and each thread
 // keeps the U units it decodes in registers from the maximum to the rounding. tpr
-// threads (whole warps) a row. Bound by instruction issue (13 an element, half of them
-// work of a row and thread): Q8_0 4096 x 11008 26.0 us, 3.58 TB/s; without its stores
-// 20.6, without its loads 23.0.
+// threads (whole warps) a row. Nothing is full: instructions (13 an element, half of them
+// work of a row and thread) take 66 % of the issue slots, memory is at 55 % of the copy
+// bandwidth, and a group's decoding, maximum and rounding wait for one another. Q8_0
+// 4096 x 11008 26.0 us, 3.58 TB/s; without its stores 20.6, without its loads 23.0.
 __device__ __forceinline__ void copy16(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n"
                  ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
@@ -763,7 +764,7 @@ extern "C" int llamini_weights_i8_device(u32 type, const void* d_blocks, u32 row
     a.scale = d_scale;
     a.row_bytes = type_bytes(type, cols);
     a.ld_q = ld_q;
-    a.rows = rows; a.cols = cols; a.type = type;
+    a.rows = rows; a.cols = cols;
     a.seg_units = kWSeg / ti.block_bytes * (ti.block_elems / 32);    // whole blocks to a segment
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     bool ok = false;
