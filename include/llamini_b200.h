@@ -163,8 +163,9 @@ int llamini_gemm_i8_device(const i8* d_a, u64 ld_a, const f32* d_a_scale, u32 ro
 /* The longest that a product's kernel waits for its own copies and tensor-core
  * products before it gives up (its outputs are NaN then), for the calls that follow from
  * any thread: 2 s unless set, at most 60 s. With 0 such a kernel gives up without
- * waiting, which shows a caller's handling of llamini_i8_status without a fault (up
- * to two tokens, and rows that are not in 16-byte pitches, have no waits to run out). */
+ * waiting, which shows a caller's handling of llamini_i8_status without a fault
+ * (products of one or two tokens, of up to eight where they take the same kernel, and
+ * from rows that are not in 16-byte pitches have no waits to run out). */
 int llamini_set_i8_wait_ns(u64 ns);
 
 /* Waits for `stream`, then 0, or -1 when a bounded wait inside a product's kernel has
